@@ -20,6 +20,8 @@ FENCE_KV_F16 = 0
 FENCE_KV_BF16 = 1
 GGML_Q8_0 = 8
 GGML_Q6_K = 14
+FENCE_F32, FENCE_F16, FENCE_BF16 = range(3)
+FENCE_KV8_INT8, FENCE_KV8_E4M3 = range(2)
 
 _c_float_p = ctypes.POINTER(ctypes.c_float)
 _c_int_p = ctypes.POINTER(ctypes.c_int)
@@ -66,6 +68,35 @@ class SynthSpec(ctypes.Structure):
         ("n_experts", ctypes.c_int), ("n_experts_used", ctypes.c_int), ("write_tokenizer", ctypes.c_int),
         ("gguf_version", ctypes.c_int), ("alignment", ctypes.c_uint32), ("seed", ctypes.c_uint64),
         ("q6k_d", ctypes.c_float), ("q8_d", ctypes.c_float), ("norm_value", ctypes.c_float),
+    ]
+
+
+class KV8Cache(ctypes.Structure):
+    """fence_kv8_cache: one layer's paged 8-bit cache (device addresses)."""
+    _fields_ = [
+        ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp),
+        ("n_pages", ctypes.c_int), ("n_kv_heads", ctypes.c_int), ("page_tokens", ctypes.c_int),
+        ("head_dim", ctypes.c_int), ("format", ctypes.c_int),
+    ]
+
+
+class PagedBatch(ctypes.Structure):
+    """fence_paged_batch: one step's batch, the plan's inputs and outputs (device addresses)."""
+    _fields_ = [
+        ("n_req", ctypes.c_int), ("n_tokens", ctypes.c_int), ("page_tokens", ctypes.c_int),
+        ("max_pages", ctypes.c_int), ("n_pages", ctypes.c_int), ("n_touch", ctypes.c_int),
+        ("ctx_len", _vp), ("new_len", _vp), ("block_table", _vp), ("free_pages", _vp), ("n_free", _vp),
+        ("n_free_out", _vp), ("ctx_out", _vp), ("kv_len", _vp), ("new_start", _vp), ("slot", _vp),
+        ("pos", _vp), ("touch", _vp),
+    ]
+
+
+class KV8Attn(ctypes.Structure):
+    """fence_kv8_attn: the operands of fence_kv8_attention (device addresses)."""
+    _fields_ = [
+        ("q", _vp), ("out", _vp), ("lse", _vp), ("q_stride", ctypes.c_longlong), ("out_stride", ctypes.c_longlong),
+        ("type", ctypes.c_int), ("n_q_heads", ctypes.c_int), ("max_new", ctypes.c_int), ("window", ctypes.c_int),
+        ("scale", ctypes.c_float), ("workspace", _vp), ("workspace_bytes", ctypes.c_size_t),
     ]
 
 
@@ -131,6 +162,15 @@ SIGNATURES = [
                                         ctypes.POINTER(ctypes.c_size_t)]),
     ("fence_format_chat", ctypes.c_int, [_vp, ctypes.c_char_p, ctypes.c_char_p, _c_int_p, ctypes.c_int, _c_int_p]),
     ("fence_chat_append", ctypes.c_int, [_vp, ctypes.c_int, ctypes.c_char_p, _c_int_p, ctypes.c_int, _c_int_p]),
+    ("fence_paged_plan", ctypes.c_int, [ctypes.POINTER(PagedBatch), _vp]),
+    ("fence_kv8_store", ctypes.c_int, [ctypes.POINTER(KV8Cache), ctypes.POINTER(PagedBatch), _vp, _vp, ctypes.c_int,
+                                       ctypes.c_longlong, ctypes.c_longlong, _vp]),
+    ("fence_kv8_load", ctypes.c_int, [ctypes.POINTER(KV8Cache), _vp, ctypes.c_int, _vp, _vp, ctypes.c_int,
+                                      ctypes.c_longlong, ctypes.c_longlong, _vp]),
+    ("fence_kv8_attention_workspace_bytes", ctypes.c_size_t,
+     [ctypes.POINTER(KV8Cache), ctypes.POINTER(PagedBatch), ctypes.POINTER(KV8Attn)]),
+    ("fence_kv8_attention", ctypes.c_int,
+     [ctypes.POINTER(KV8Cache), ctypes.POINTER(PagedBatch), ctypes.POINTER(KV8Attn), _vp]),
 ]
 
 _lib = None

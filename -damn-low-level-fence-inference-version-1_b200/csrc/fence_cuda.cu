@@ -8,3 +8,6 @@
 #include "sampler_dev.cu"
 #include "prefill.cu"
 #include "engine.cu"
+#include "paged_plan.cu"
+#include "kv8_store.cu"
+#include "kv8_attn.cu"

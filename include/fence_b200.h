@@ -53,7 +53,8 @@ typedef struct CUstream_st* fence_stream_t;
 /* Thread-local text of the last error raised by any fence_* call on this thread ("" if none). */
 const char* fence_last_error(void);
 /* Returns and clears the device-side error word that kernels set when a bounded wait expires
- * (0 if none). Synchronises the device. */
+ * (FENCE_E_DEVICE_WAIT), or when a paged batch (section 5) holds a length, a page id or a slot out of
+ * range (FENCE_E_ARG; that access is left out). 0 if none. Synchronises the device. */
 int fence_device_error(void);
 
 /* ---- quant block types (byte-identical to the reference) ---- */
@@ -404,6 +405,118 @@ int fence_format_chat(fence_tokenizer* t, const char* system_prompt, const char*
 #define FENCE_TURN_END       4
 int fence_chat_append(fence_tokenizer* t, int turn, const char* content, int* tokens, int cap,
                       int* n_inout);
+
+/* =====================================================================================
+ * 5. Batched serving over a paged 8-bit KV cache. No counterpart in the reference, whose loop
+ *    serves one request over a contiguous fp16 cache.
+ *
+ *    One step of a batch: fence_paged_plan turns the requests' lengths into block tables and slot
+ *    maps on the device; then, in every layer, fence_kv8_store quantises the step's K/V rows into the
+ *    layer's pages and fence_kv8_attention attends over them. fence_kv8_load reads rows back.
+ *    All pointers are device pointers owned by the caller, all calls are asynchronous on `stream`,
+ *    allocate nothing and never copy to the host (so a step can be captured in a graph).
+ *
+ *    A page holds page_tokens (16, 32, 64 or 128) consecutive positions of one request. A layer's
+ *    cache is the codes of K and V, [n_pages][n_kv_heads][page_tokens][head_dim] bytes each, and a
+ *    float scale for each page and head; a value is code * scale. One block table serves all layers.
+ * ===================================================================================== */
+
+/* element types of the activations (q, k, v, outputs) */
+#define FENCE_F32  0
+#define FENCE_F16  1
+#define FENCE_BF16 2
+
+/* code formats: int8 -127..127 (scale = largest |x| of the page / 127), or the 8-bit float with 4
+ * exponent and 3 mantissa bits (largest |x| / 448) */
+#define FENCE_KV8_INT8 0
+#define FENCE_KV8_E4M3 1
+
+typedef struct fence_kv8_cache {   /* one layer's cache */
+    void*  k;                      /* codes, 16-byte aligned                                     */
+    void*  v;
+    float* k_scale;                /* [n_pages][n_kv_heads], >= 0                                */
+    float* v_scale;
+    int n_pages, n_kv_heads, page_tokens;
+    int head_dim;                  /* 64, 128 or 256                                             */
+    int format;                    /* FENCE_KV8_*                                                */
+} fence_kv8_cache;
+
+typedef struct fence_paged_batch { /* one step's batch; the plan's inputs and outputs (int32)     */
+    int n_req;                     /* requests, at most FENCE_PAGED_MAX_REQ                      */
+    int n_tokens;                  /* rows of the step's token buffers (>= the new tokens' sum)  */
+    int page_tokens;
+    int max_pages;                 /* entries per row of block_table                             */
+    int n_pages;                   /* pages of the pool                                          */
+    int n_touch;                   /* rows of touch: min(n_tokens, 2 n_req + n_tokens / page_tokens) */
+    /* in */
+    const int* ctx_len;            /* [n_req] tokens each request has in the cache               */
+    const int* new_len;            /* [n_req] tokens it brings now; negative: it has ended       */
+    int* block_table;              /* [n_req][max_pages] page ids; the plan adds the new entries  */
+    int* free_pages;               /* [n_pages] stack of free pages, entries 0 .. *n_free - 1    */
+    const int* n_free;             /* [1]                                                        */
+    /* out */
+    int* n_free_out;               /* [1] the next step's n_free                                 */
+    int* ctx_out;                  /* [n_req] the next step's ctx_len                            */
+    int* kv_len;                   /* [n_req] tokens in the cache with the new ones; 0: not placed */
+    int* new_start;                /* [n_req + 1] first row of each request in the token buffers */
+    int* slot;                     /* [n_tokens] page * page_tokens + row of each token, or -1   */
+    int* pos;                      /* [n_tokens] its position, or -1                             */
+    int* touch;                    /* [n_touch][4] page, first row, first token, rows; page -1: none */
+} fence_paged_batch;
+#define FENCE_PAGED_MAX_REQ 4096
+
+/* The step's plan. The requests' tokens lie one after another in the token buffers (k, v, q) in
+ * request order, new_len[r] rows each. A request is placed if ctx + new fits max_pages and the pool:
+ * pages are handed out in request order from the top of the stack, after the pages of the ended
+ * requests (in request order, first page first) were put on it; once the pool has run out, no later
+ * request that needs a page is placed. One that is not placed keeps its ctx (ctx_out), has kv_len 0
+ * and slots -1: its rows are neither stored nor attended (their output is 0), and it may come again
+ * in a later step. An ended request's ctx_out is 0. ctx_out, kv_len and n_free_out must not be the
+ * buffers that are read (two sets, used in turn, or a copy after the step). */
+int fence_paged_plan(const fence_paged_batch* b, fence_stream_t stream);
+
+/* Stores the step's rows of K and V: k[t * k_stride + h * head_dim + i] (strides in elements, type
+ * FENCE_F32 / F16 / BF16) for the tokens of b->touch. Where a page's largest |x| grows, its scale
+ * grows with it and its older rows are brought to the new scale (one rounding); a page whose row 0 is
+ * written starts anew. scale = largest * (1 / 127 or 1 / 448), code = round(x * (1 / scale)) to
+ * nearest, ties to even; scales below the smallest normal float are stored as 0 (all codes 0). NaN or
+ * infinity in a page's rows make the page's scale NaN or infinite for that head and its codes 0, so
+ * attention over it gives NaN. A page must be written by one request at a time. */
+int fence_kv8_store(const fence_kv8_cache* c, const fence_paged_batch* b, const void* k, const void* v,
+                    int type, long long k_stride, long long v_stride, fence_stream_t stream);
+
+/* Rows slot[0 .. n) of the cache as values: k[i * k_stride + h * head_dim + e] = code * scale, the
+ * same for v (either may be NULL). Rows of slot -1 are 0. */
+int fence_kv8_load(const fence_kv8_cache* c, const int* slot, int n, void* k, void* v, int type,
+                   long long k_stride, long long v_stride, fence_stream_t stream);
+
+typedef struct fence_kv8_attn {
+    const void* q;                 /* q[t * q_stride + head * head_dim + i]                      */
+    void* out;                     /* out[t * out_stride + head * head_dim + i]                  */
+    float* lse;                    /* [n_tokens][n_q_heads] log of the sum of exp(score), or NULL */
+    long long q_stride, out_stride;/* elements                                                   */
+    int type;                      /* of q and out: FENCE_F32 / F16 / BF16                       */
+    int n_q_heads;                 /* a multiple of n_kv_heads; head h reads kv head h / (Hq/Hkv) */
+    int max_new;                   /* the most new tokens that a request brings (a hint for the
+                                      choice of kernel: results do not depend on it beyond rounding) */
+    int window;                    /* > 0: a query sees the last `window` positions only          */
+    float scale;                   /* of the scores, e.g. 1 / sqrt(head_dim)                     */
+    void* workspace;               /* fence_kv8_attention_workspace_bytes, 256-byte aligned; zeroed once
+                                      by the caller before its first use, left ready by every call  */
+    size_t workspace_bytes;
+} fence_kv8_attn;
+
+/* Causal grouped-query attention of the batch: of request r's n = new_start[r+1] - new_start[r] rows,
+ * row i is at position kv_len[r] - n + i and sees the positions 0 .. that one (the last `window`)
+ * through block_table[r]. Uses b->n_req, n_tokens, max_pages, block_table, kv_len and new_start. Rows
+ * that see nothing (a request that is not placed, rows after the last request's) give 0 and lse -inf.
+ * Codes enter the products exactly, q and the softmax weights as fp16 (fp32 q: as a pair of fp16);
+ * sums are fp32. The result does not depend on timing. Calls that overlap in time need workspaces of
+ * their own. */
+size_t fence_kv8_attention_workspace_bytes(const fence_kv8_cache* c, const fence_paged_batch* b,
+                                           const fence_kv8_attn* a);
+int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_batch* b, const fence_kv8_attn* a,
+                        fence_stream_t stream);
 
 #ifdef __cplusplus
 } /* extern "C" */
