@@ -1,0 +1,652 @@
+// kv8_decode.cuh — attention of a few query rows per request over the paged 8-bit cache (decode, drafts).
+//
+//   s[j][h] = (K code row j . q row h) * k_scale[page] * scale,  p = softmax(s),  out = p . (V code rows * v_scale[page])
+//
+// Bound: HBM, two bytes per key, head and channel; the kernel has to keep the codes coming and turn them
+// into matrix operands fast enough.
+//
+//  * Work is the list of 64-key tiles of every (request, KV head, group of 8 NT query rows), cut into
+//    equal runs, one per CTA, whatever the lengths are: a CTA's run may begin and end inside a unit. Such a
+//    unit's partial results go to the workspace and the last of its CTAs to arrive joins them in the
+//    order of the keys, so the result does not depend on timing.
+//  * One producer warp per CTA copies each tile's pages (TMA, 16 or more rows at a time, swizzled so
+//    that all operand loads are free of bank conflicts) and their scales into a ring of stages.
+//  * Four consumer warps take 16 keys of a tile each, with a softmax state of their own: keys are the
+//    rows of the matrix products (S^T = K Q^T: 16 keys x 8 rows, O^T = V^T P^T: 16 channels x 8 rows),
+//    so 8 query rows fill the instruction and nothing is padded for grouped heads. A page holds 16 or
+//    more keys: a warp's scales are two numbers.
+//  * Codes become fp16 exactly. Scales never touch them: k_scale multiplies the scores, v_scale / (the
+//    largest v_scale so far) the weights. q rows are brought to [256, 512) by a power of two, so that
+//    fp16 holds them whatever their range. SPLIT (fp32 activations): q and the weights as a pair of
+//    fp16 (22 bits), and the products of 16 keys are added to the sums in fp32 outside the matrix unit.
+#pragma once
+
+#include <cuda.h>
+
+#include "kv8.cuh"
+
+namespace fence {
+
+struct KAttnArgs {
+    fence_kv8_cache c;
+    const int* block_table;
+    const int* kv_len;
+    const int* new_start;
+    int n_req, n_tokens, max_pages, shift, G, n_q_heads, window, type;
+    const void* q;
+    void* out;
+    float* lse;
+    long long q_stride, out_stride;
+    float scale_log2;  // scale * log2(e): scores are kept as exponents of 2
+    int max_rows;      // requests of more query rows per KV head are left to the other kernel
+    int* arrived;      // [CTAs] partial results of the unit that starts in this CTA and goes on in the next
+    float* part;       // [CTAs][2][rows * (head_dim + 2)]
+};
+
+constexpr int KD_TILE = 64, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
+constexpr int KD_MIN_TILES = 2;  // tiles per CTA below which more CTAs only add joins
+constexpr float KD_LAZY = 8.f;   // the running maximum may lag by 2^8: fp16 weights stay below 2^16
+
+template <int HD, int NT>
+struct KDShape {
+    static constexpr int CTAS = HD == 256 && NT == 2 ? 1 : 2;  // per SM; one where the sums take 128 registers
+    static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 6 : NT == 2 ? 5 : 3;
+    static constexpr int KV_BYTES = KD_TILE * HD;
+    static constexpr int STAGE = 2 * KV_BYTES;
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int SLAB = HD + 4;
+    // after the ring: scales, barriers, q fragments (high and low), rows' scales, the warps' (m, l), the slab
+    static constexpr int O_SCALE = STAGES * STAGE;
+    static constexpr int O_BAR = O_SCALE + STAGES * 32;
+    static constexpr int O_Q = O_BAR + 2 * STAGES * 8;
+    static constexpr int O_QS = O_Q + NT * 2 * (HD / 16) * 256;
+    static constexpr int O_ML = O_QS + ROWS * 4;
+    static constexpr int O_SLAB = O_ML + KD_WARPS * ROWS * 8;
+    static constexpr int O_SCAN = O_SLAB + ROWS * SLAB * 4;
+    static constexpr int SMEM = O_SCAN + 64 + 1024;  // + the prefix sums [n_req + 1], + alignment
+};
+
+// two codes (bytes lo and lo + 1 of w) -> two fp16, exactly
+template <int FMT>
+__device__ __forceinline__ uint32_t kd_half2(uint32_t w, bool high) {
+    if (FMT == KV8_INT8) {
+        // w holds code + 128: bytes beside 0x64 are the fp16 numbers 1024 + byte; less 1152
+        const uint32_t x = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? w >> 16 : w & 0xffffu), __NV_E4M3);
+    return (uint32_t)r.x | ((uint32_t)r.y << 16);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t kd_bias(uint32_t w) { return FMT == KV8_INT8 ? w ^ 0x80808080u : w; }
+
+__device__ __forceinline__ void kd_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t kd_transpose(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float kd_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t kd_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// what fp16 leaves of a and b
+__device__ __forceinline__ uint32_t kd_pack_rest(float a, float b, uint32_t hi) {
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return kd_pack(a - h.x, b - h.y);
+}
+__device__ __forceinline__ uint2 kd_lds64(uint32_t sa) {
+    uint2 v;
+    asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(sa));
+    return v;
+}
+__device__ __forceinline__ void kd_tma(uint32_t dst, const CUtensorMap* tm, int x, int y, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(tm)), "r"(x), "r"(y), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// What one request contributes: its rows in the token buffers and the keys that they can see.
+struct KReq {
+    int start, n, kv, tile0, tiles, groups;
+};
+__device__ __forceinline__ KReq kd_request(const KAttnArgs& a, int r, int rows_per_group, int tile_keys, bool report) {
+    KReq q{};
+    q.start = a.new_start[r];
+    int end = a.new_start[r + 1], kv = a.kv_len[r];
+    const int most = a.max_pages << a.shift;
+    if (q.start < 0 || end < q.start || end > a.n_tokens || kv < 0 || kv > most) {
+        if (report) set_device_error(KV8_BAD);
+        q.start = max(0, min(q.start, a.n_tokens));
+        end = max(q.start, min(end, a.n_tokens));
+        kv = max(0, min(kv, most));
+    }
+    q.n = end - q.start;
+    q.kv = kv;
+    if (q.n == 0) return q;
+    const int lo = a.window > 0 ? max(0, kv - q.n - a.window + 1) : 0;  // the first row's first key
+    q.tile0 = lo / tile_keys;
+    q.tiles = kv > 0 ? (kv - 1) / tile_keys - q.tile0 + 1 : 1;  // a request that sees nothing still has its rows written
+    q.groups = (int)(((long long)q.n * a.G + rows_per_group - 1) / rows_per_group);
+    return q;
+}
+
+template <int FMT, int HD, bool SPLIT, int NT>
+__global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
+    kv8_decode_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    using S = KDShape<HD, NT>;
+    constexpr int ROWS = S::ROWS, KS = HD / 16, MT = HD / 16, HALVES = HD == 256 ? 2 : 1, LINE = HD == 64 ? 64 : 128;
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    const uint32_t sbase = smem_u32(smem);
+    float* s_scale = reinterpret_cast<float*>(smem + S::O_SCALE);  // [stage][K 4, V 4]
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::O_BAR);
+    uint64_t* empty = full + S::STAGES;
+    uint2* s_q = reinterpret_cast<uint2*>(smem + S::O_Q);  // [NT][high, low][KS][32]
+    float* s_qs = reinterpret_cast<float*>(smem + S::O_QS);
+    float2* s_ml = reinterpret_cast<float2*>(smem + S::O_ML);  // [warp][ROWS]
+    float* s_slab = reinterpret_cast<float*>(smem + S::O_SLAB);
+    int* s_misc = reinterpret_cast<int*>(smem + S::O_SCAN);
+    int* s_pre = s_misc + 16;  // [n_req + 1] tiles before each request
+
+    if (tid == 0) {
+        for (int s = 0; s < S::STAGES; ++s) {
+            mbar_init(&full[s], 33);
+            mbar_init(&empty[s], KD_WARPS);
+        }
+        fence_barrier_init();
+    }
+    // ---- prefix sums of the requests' tiles
+    {
+        const int per = (a.n_req + KD_THREADS - 1) / KD_THREADS;
+        const int r0 = min(a.n_req, tid * per), r1 = min(a.n_req, r0 + per);
+        long long sum = 0;
+        for (int r = r0; r < r1; ++r) {
+            const KReq q = kd_request(a, r, ROWS, KD_TILE, blockIdx.x == 0);
+            const long long w = (long long)q.n * a.G > a.max_rows ? 0 : (long long)q.tiles * q.groups * a.c.n_kv_heads;
+            s_pre[r] = (int)min(w, (long long)INT_MAX);
+            sum += w;
+        }
+        long long v = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, v, o);
+            if (lane >= o) v += u;
+        }
+        long long* s_w = reinterpret_cast<long long*>(s_ml);
+        if (lane == 31) s_w[warp] = v;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) v += s_w[w];
+        v -= sum;
+        for (int r = r0; r < r1; ++r) {
+            const int w = s_pre[r];
+            s_pre[r] = (int)min(v, (long long)INT_MAX);
+            v += w;
+        }
+        if (tid == KD_THREADS - 1) {
+            if (v > INT_MAX) set_device_error(KV8_BAD);
+            s_pre[a.n_req] = (int)min(v, (long long)INT_MAX);
+        }
+        __syncthreads();
+    }
+    const int total = s_pre[a.n_req];
+    const int per = max(KD_MIN_TILES, (int)(((long long)total + gridDim.x - 1) / gridDim.x));
+    const int begin = (int)min((long long)total, (long long)blockIdx.x * per), end = min(total, begin + min(per, total - begin));
+    // the request of the run's first tile
+    int r = 0;
+    {
+        int hi = a.n_req;
+        while (hi - r > 1) {
+            const int mid = (r + hi) >> 1;
+            if (s_pre[mid] <= begin) r = mid;
+            else hi = mid;
+        }
+    }
+    bool ok = true;
+    const int P = a.c.page_tokens, box = min(P, KD_TILE), boxes = KD_TILE / box;
+
+    if (warp == KD_WARPS) {
+        // ---------------------------------------------------------------- producer
+        int it = 0;
+        for (int cur = begin; cur < end;) {
+            while (s_pre[r + 1] <= cur) ++r;
+            const KReq q = kd_request(a, r, ROWS, KD_TILE, false);
+            const int unit = (cur - s_pre[r]) / q.tiles, first = (cur - s_pre[r]) - unit * q.tiles;
+            const int cnt = min(q.tiles - first, end - cur), h = unit / q.groups;
+            const int lo = a.window > 0 ? max(0, q.kv - q.n - a.window + 1) : 0;
+            const int* table = a.block_table + (size_t)r * a.max_pages;
+            int ids = 0, ids_at = -1;  // this lane's page id of a run of 32 pages
+            for (int i = 0; i < cnt; ++i, ++it) {
+                const int s = it % S::STAGES, key0 = (q.tile0 + first + i) * KD_TILE;
+                const int p0 = key0 >> a.shift;
+                if (ids_at < 0 || p0 >= ids_at + 32 || p0 < ids_at) {
+                    ids_at = p0 & ~(boxes - 1);
+                    const int j = ids_at + lane;
+                    ids = (j << a.shift) < q.kv ? table[j] : 0;
+                }
+                if (ok && it >= S::STAGES) ok = mbar_wait(&empty[s], (uint32_t)(it / S::STAGES - 1) & 1u);
+                if (!__all_sync(0xffffffffu, ok)) {
+                    ok = false;
+                    break;
+                }
+                int page = __shfl_sync(0xffffffffu, ids, (p0 - ids_at + lane) & 31);
+                const int k_lo = key0 + lane * box;
+                bool mine = lane < boxes && k_lo < q.kv && k_lo + box > lo;
+                if (mine && (page < 0 || page >= a.c.n_pages)) {
+                    set_device_error(KV8_BAD);
+                    page = 0;
+                }
+                const int loads = __popc(__ballot_sync(0xffffffffu, mine));
+                if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)(loads * box * HD * 2));
+                __syncwarp();
+                if (mine) {
+                    const int unit_row = page * a.c.n_kv_heads + h;
+                    const int y = unit_row * P + (k_lo & (P - 1));
+                    const uint32_t dst = sbase + (uint32_t)(s * S::STAGE + lane * box * LINE);
+#pragma unroll
+                    for (int x = 0; x < HALVES; ++x) {
+                        kd_tma(dst + x * KD_TILE * LINE, &tm_k, x * 128, y, &full[s]);
+                        kd_tma(dst + S::KV_BYTES + x * KD_TILE * LINE, &tm_v, x * 128, y, &full[s]);
+                    }
+                    cp_async4(s_scale + s * 8 + lane, a.c.k_scale + unit_row);
+                    cp_async4(s_scale + s * 8 + 4 + lane, a.c.v_scale + unit_row);
+                }
+                asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
+            }
+            if (!ok) break;
+            cur += cnt;
+        }
+        cp_async_wait_all();
+        return;
+    }
+    // -------------------------------------------------------------------- consumers
+    // rows that belong to no request
+    {
+        const int used = max(0, min(a.new_start[a.n_req], a.n_tokens));
+        const long long row = (long long)a.n_q_heads * HD, n = (a.n_tokens - used) * row;
+        const int ct = blockIdx.x * 128 + tid, cs = gridDim.x * 128;
+        for (long long i = ct; i < n; i += cs) kv8_st1(a.out, (used + i / row) * a.out_stride + i % row, a.type, 0.f);
+        if (a.lse)
+            for (long long i = ct; i < (long long)(a.n_tokens - used) * a.n_q_heads; i += cs)
+                a.lse[(long long)used * a.n_q_heads + i] = -INFINITY;
+    }
+    int it = 0;
+    for (int cur = begin; cur < end;) {
+        while (s_pre[r + 1] <= cur) ++r;
+        const KReq q = kd_request(a, r, ROWS, KD_TILE, false);
+        const int unit = (cur - s_pre[r]) / q.tiles, first = (cur - s_pre[r]) - unit * q.tiles;
+        const int cnt = min(q.tiles - first, end - cur), h = unit / q.groups, row0 = (unit - h * q.groups) * ROWS;
+        const int rows = min(ROWS, q.n * a.G - row0);  // row = token * G + head in the group
+        // ---- q rows: scaled by a power of two into [256, 512), as B fragments
+        for (int i = warp; i < ROWS; i += KD_WARPS) {
+            constexpr int EPL = HD / 32;  // elements per lane: 2, 4 or 8
+            float x[EPL];
+            uint32_t big = 0;
+            const int tok = q.start + (row0 + i) / a.G, head = h * a.G + (row0 + i) % a.G;
+            const long long at = tok * a.q_stride + (long long)head * HD + lane * EPL;
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) {
+                x[e] = i >= rows ? 0.f
+                       : a.type == FENCE_F32 ? static_cast<const float*>(a.q)[at + e]
+                       : a.type == FENCE_F16 ? __half2float(static_cast<const __half*>(a.q)[at + e])
+                                             : __bfloat162float(static_cast<const __nv_bfloat16*>(a.q)[at + e]);
+                big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
+            }
+            big = __reduce_max_sync(0xffffffffu, big);
+            const int ex = (int)(big >> 23);  // biased exponent
+            const bool plain = ex == 255;     // infinity or NaN in the row
+            const int sh = plain ? 0 : max(ex, 1) - 127 - 8;  // times 2^-sh
+            const float f1 = __uint_as_float((uint32_t)(127 - max(min(sh, 126), -126)) << 23);
+            const float f2 = sh > 126 ? 0.5f : sh < -126 ? __uint_as_float((uint32_t)(127 - sh - 126) << 23) : 1.f;
+            if (lane == 0) s_qs[i] = plain ? 1.f : ldexpf(1.f, sh);
+#pragma unroll
+            for (int e = 0; e < EPL; e += 2) {
+                const float u = x[e] * f1 * f2, v = x[e + 1] * f1 * f2;
+                const uint32_t hi = kd_pack(u, v);
+                const int c = lane * EPL + e;  // channel: k step j, thread ct of the quad, pair
+                const int half = c / 128, cc = c % 128;
+                const int ct = HD == 64 ? cc / 16 : cc / 32, j = HD == 64 ? (cc % 16) / 4 : half * 8 + (cc % 32) / 4;
+                uint32_t* dst = reinterpret_cast<uint32_t*>(s_q) +
+                                ((((i >> 3) * 2) * KS + j) * 32 + (i & 7) * 4 + ct) * 2 + ((c >> 1) & 1);
+                dst[0] = hi;
+                if (SPLIT) dst[KS * 64] = kd_pack_rest(u, v, hi);
+            }
+        }
+        named_bar_sync(1, 32 * KD_WARPS);
+        // ---- this thread's rows 8 nt + 2 t + e: scale and last visible position
+        float qs[NT][2], m[NT][2], l[NT][2];
+        int lim[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int i = nt * 8 + 2 * t + e;
+                qs[nt][e] = s_qs[i] * a.scale_log2;
+                lim[nt][e] = i < rows ? q.kv - q.n + (row0 + i) / a.G : -1;
+                m[nt][e] = -INFINITY;
+                l[nt][e] = 0.f;
+            }
+        // keys that every row sees, and keys that some row sees
+        const int lim_first = q.kv - q.n + row0 / a.G, lim_last = q.kv - q.n + (row0 + rows - 1) / a.G;
+        const int all_lo = a.window > 0 ? lim_last - a.window + 1 : 0, any_lo = a.window > 0 ? lim_first - a.window + 1 : 0;
+        const bool full_rows = rows == ROWS;
+        float o[MT][NT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+        float vref = 0.f, vinv = 0.f;
+
+        for (int i = 0; i < cnt; ++i, ++it) {
+            const int s = it % S::STAGES, key0 = (q.tile0 + first + i) * KD_TILE + warp * 16;
+            if (ok) ok = mbar_wait(&full[s], (uint32_t)(it / S::STAGES) & 1u);
+            __syncwarp();
+            if (key0 <= lim_last && key0 + 15 >= any_lo && lim_last >= 0) {
+                const uint32_t kb = sbase + (uint32_t)(s * S::STAGE), vb = kb + S::KV_BYTES;
+                const int pi = (warp * 16) / box;
+                const float sk = s_scale[s * 8 + pi], sv = s_scale[s * 8 + 4 + pi];
+                // ---- scores of 16 keys
+                float acc[NT][2][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) acc[nt][c][0] = acc[nt][c][1] = acc[nt][c][2] = acc[nt][c][3] = 0.f;
+                const int ra = warp * 16 + g;
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c) {  // 16 bytes of each of the rows g and g + 8
+                    const uint32_t off = HD == 64 ? (uint32_t)(ra * 64 + ((t ^ ((ra >> 1) & 3)) << 4))
+                                                  : (uint32_t)((c >> 1) * KD_TILE * 128 + ra * 128 + (((2 * t + (c & 1)) ^ g) << 4));
+                    const uint4 ka = lds128(kb + off), kc = lds128(kb + off + 8 * LINE);
+                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kc.x, kc.y, kc.z, kc.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int j = HD == 64 ? w : (c >> 1) * 8 + (c & 1) * 4 + w;
+                        const uint32_t xa = kd_bias<FMT>(wa[w]), xb = kd_bias<FMT>(wb[w]);
+                        const uint32_t a0 = kd_half2<FMT>(xa, false), a1 = kd_half2<FMT>(xb, false);
+                        const uint32_t a2 = kd_half2<FMT>(xa, true), a3 = kd_half2<FMT>(xb, true);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            const uint2 b = s_q[((nt * 2) * KS + j) * 32 + lane];
+                            kd_mma(acc[nt][SPLIT ? 0 : w & 1], a0, a1, a2, a3, b.x, b.y);
+                            if (SPLIT) {
+                                const uint2 bl = s_q[((nt * 2 + 1) * KS + j) * 32 + lane];
+                                kd_mma(acc[nt][1], a0, a1, a2, a3, bl.x, bl.y);
+                            }
+                        }
+                    }
+                }
+                // ---- scale, mask, the largest of each row
+                const bool masked = !full_rows || key0 + 15 > lim_first || (a.window > 0 && key0 < all_lo);
+                float p[NT][4];
+                bool move = sv > vref;
+                float mt[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float f = qs[nt][e & 1] * sk;
+                        float x = (acc[nt][0][e] + acc[nt][1][e]) * f;
+                        if (masked) {
+                            const int key = key0 + g + (e >> 1) * 8, li = lim[nt][e & 1];
+                            if (key > li || (a.window > 0 && key <= li - a.window)) x = -INFINITY;
+                        }
+                        p[nt][e] = x;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float x = fmaxf(p[nt][e], p[nt][e + 2]);
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        mt[nt][e] = x;
+                        move |= x > m[nt][e] + KD_LAZY;  // also the first: m = -inf
+                    }
+                }
+                if (__any_sync(0xffffffffu, move)) {
+                    float vf = 1.f;
+                    if (sv > vref) {
+                        vinv = 1.f / sv;
+                        vf = vref * vinv;
+                        vref = sv;
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float mn = fmaxf(m[nt][e], mt[nt][e]);
+                            const float al = mn == -INFINITY ? 1.f : kd_exp2(m[nt][e] - mn);
+                            m[nt][e] = mn;
+                            l[nt][e] *= al;
+#pragma unroll
+                            for (int i2 = 0; i2 < MT; ++i2) {
+                                o[i2][nt][e] *= al * vf;
+                                o[i2][nt][e + 2] *= al * vf;
+                            }
+                        }
+                }
+                const float fv = vref > 0.f ? sv * vinv : sv == 0.f ? 1.f : sv;  // NaN stays NaN
+                uint32_t b0[NT], b1[NT], c0[NT], c1[NT];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float mm = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+                        const float x = kd_exp2(p[nt][e] - mm);
+                        l[nt][e & 1] += x;
+                        p[nt][e] = x * fv;
+                    }
+                    const uint32_t h0 = kd_pack(p[nt][0], p[nt][1]), h1 = kd_pack(p[nt][2], p[nt][3]);
+                    b0[nt] = kd_transpose(h0);
+                    b1[nt] = kd_transpose(h1);
+                    if (SPLIT) {
+                        c0[nt] = kd_transpose(kd_pack_rest(p[nt][0], p[nt][1], h0));
+                        c1[nt] = kd_transpose(kd_pack_rest(p[nt][2], p[nt][3], h1));
+                    }
+                }
+                // ---- O^T += V^T P^T; keys that no row sees count as zero, whatever their codes are
+                const int rv = warp * 16 + 2 * t;
+                uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+                if (masked) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0 + 2 * t + (e & 1) + (e >> 1) * 8;
+                        keep[e] = key <= lim_last && key >= any_lo ? ~0u : 0u;
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < HALVES; ++x) {
+                    constexpr int WORDS = HD == 64 ? 2 : 4;
+                    uint32_t w[4][4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int row = rv + (e & 1) + (e >> 1) * 8;
+                        if (HD == 64) {
+                            const uint2 v = kd_lds64(vb + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + ((g & 1) << 3));
+                            w[e][0] = v.x, w[e][1] = v.y;
+                        } else {
+                            const uint4 v = lds128(vb + x * KD_TILE * 128 + row * 128 + ((g ^ (row & 7)) << 4));
+                            w[e][0] = v.x, w[e][1] = v.y, w[e][2] = v.z, w[e][3] = v.w;
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int k = 0; k < WORDS; ++k) w[e][k] &= keep[e];
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < WORDS; ++k) {
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {  // bytes 0, 1 or 2, 3 of the word: two channels
+                            const uint32_t sel = y ? 0x7362 : 0x5140;
+                            const uint32_t u = kd_bias<FMT>(__byte_perm(w[0][k], w[1][k], sel));
+                            const uint32_t v = kd_bias<FMT>(__byte_perm(w[2][k], w[3][k], sel));
+                            const uint32_t a0 = kd_half2<FMT>(u, false), a1 = kd_half2<FMT>(u, true);
+                            const uint32_t a2 = kd_half2<FMT>(v, false), a3 = kd_half2<FMT>(v, true);
+                            const int i2 = x * 8 + 2 * k + y;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                if (SPLIT) {
+                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                    kd_mma(d, a0, a1, a2, a3, c0[nt], c1[nt]);
+                                    kd_mma(d, a0, a1, a2, a3, b0[nt], b1[nt]);
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) o[i2][nt][e] += d[e];
+                                } else {
+                                    kd_mma(o[i2][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
+        }
+        // ---- the four warps' results into one: largest m, then sum of o * v_ref * 2^(m - M)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = l[nt][e];
+                x += __shfl_xor_sync(0xffffffffu, x, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g == 0) s_ml[warp * ROWS + nt * 8 + 2 * t + e] = make_float2(m[nt][e], x);
+            }
+        named_bar_sync(1, 32 * KD_WARPS);
+        float w_row[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < KD_WARPS; ++w) M = fmaxf(M, s_ml[w * ROWS + nt * 8 + 2 * t + e].x);
+                w_row[nt][e] = kd_exp2(m[nt][e] - (M == -INFINITY ? 0.f : M)) * vref;
+            }
+        for (int w = 0; w < KD_WARPS; ++w) {
+            if (w == warp) {
+#pragma unroll
+                for (int i2 = 0; i2 < MT; ++i2)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            // columns in the order (channel tile, g, 2 channels)
+                            float2* d = reinterpret_cast<float2*>(s_slab + (nt * 8 + 2 * t + e) * S::SLAB + i2 * 16 + 2 * g);
+                            float2 v = make_float2(o[i2][nt][e] * w_row[nt][e], o[i2][nt][e + 2] * w_row[nt][e]);
+                            if (w > 0) {
+                                const float2 u = *d;
+                                v.x += u.x;
+                                v.y += u.y;
+                            }
+                            *d = v;
+                        }
+            }
+            named_bar_sync(1, 32 * KD_WARPS);
+        }
+        // channel of slab column c
+        auto channel = [](int c) {
+            const int i2 = c >> 4, gg = (c >> 1) & 7, e = c & 1;
+            return HD == 64 ? gg * 8 + 2 * i2 + e : (i2 >> 3) * 128 + gg * 16 + 2 * (i2 & 7) + e;
+        };
+        const bool whole = cnt == q.tiles;
+        const int unit0 = cur - first;  // the unit's first tile in the list
+        const int c_first = unit0 / per, c_last = (unit0 + q.tiles - 1) / per;
+        const int stride = ROWS * (HD + 2);
+        bool write = whole;
+        if (!whole) {
+            float* rec = a.part + ((long long)blockIdx.x * 2 + (first > 0 ? 0 : 1)) * stride;
+            for (int i = tid; i < ROWS * (HD / 4); i += 128) {
+                const int row = i / (HD / 4), c = (i % (HD / 4)) * 4;
+                const float* s4 = s_slab + row * S::SLAB + c;
+                __stcg(reinterpret_cast<float4*>(rec + row * HD + c), make_float4(s4[0], s4[1], s4[2], s4[3]));
+            }
+            if (tid < ROWS) {
+                float M = -INFINITY, L = 0.f;
+                for (int w = 0; w < KD_WARPS; ++w) M = fmaxf(M, s_ml[w * ROWS + tid].x);
+                for (int w = 0; w < KD_WARPS; ++w) {
+                    const float2 v = s_ml[w * ROWS + tid];
+                    L += v.y * kd_exp2(v.x - (M == -INFINITY ? 0.f : M));
+                }
+                __stcg(reinterpret_cast<float2*>(rec + ROWS * HD) + tid, make_float2(M, L));
+            }
+            __threadfence();
+            named_bar_sync(1, 32 * KD_WARPS);
+            if (tid == 0) {
+                const int n = atomicAdd(a.arrived + c_first, 1);
+                const bool last = n == c_last - c_first;
+                if (last) a.arrived[c_first] = 0;  // ready for the next call
+                __threadfence();
+                s_misc[0] = last;
+            }
+            named_bar_sync(1, 32 * KD_WARPS);
+            write = s_misc[0] != 0;
+            if (write) {
+                // join the parts in the order of the keys
+                for (int i = tid; i < ROWS * (HD / 4); i += 128) {
+                    const int row = i / (HD / 4), c = (i % (HD / 4)) * 4;
+                    float M = -INFINITY, L = 0.f;
+                    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int k = c_first; k <= c_last; ++k) {
+                        const float* pr = a.part + ((long long)k * 2 + (k == c_first ? 1 : 0)) * stride;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(pr + ROWS * HD) + row);
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(pr + row * HD + c));
+                        const float mn = fmaxf(M, ml.x), mm = mn == -INFINITY ? 0.f : mn;
+                        const float al = kd_exp2(M - mm), be = kd_exp2(ml.x - mm);
+                        M = mn;
+                        L = L * al + ml.y * be;
+                        sum.x = sum.x * al + v.x * be;
+                        sum.y = sum.y * al + v.y * be;
+                        sum.z = sum.z * al + v.z * be;
+                        sum.w = sum.w * al + v.w * be;
+                    }
+                    float* s4 = s_slab + row * S::SLAB + c;
+                    s4[0] = sum.x, s4[1] = sum.y, s4[2] = sum.z, s4[3] = sum.w;
+                    if (c == 0) {
+                        s_ml[row] = make_float2(M, L);
+#pragma unroll
+                        for (int w = 1; w < KD_WARPS; ++w) s_ml[w * ROWS + row] = make_float2(-INFINITY, 0.f);
+                    }
+                }
+                named_bar_sync(1, 32 * KD_WARPS);
+            }
+        }
+        if (write) {
+            for (int i = warp; i < rows; i += KD_WARPS) {
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int w = 0; w < KD_WARPS; ++w) M = fmaxf(M, s_ml[w * ROWS + i].x);
+#pragma unroll
+                for (int w = 0; w < KD_WARPS; ++w) {
+                    const float2 v = s_ml[w * ROWS + i];
+                    L += v.y * kd_exp2(v.x - (M == -INFINITY ? 0.f : M));
+                }
+                const int tok = q.start + (row0 + i) / a.G, head = h * a.G + (row0 + i) % a.G;
+                const float inv = L == 0.f ? 0.f : 1.f / L;
+                for (int c = lane; c < HD; c += 32)
+                    kv8_st1(a.out, tok * a.out_stride + (long long)head * HD + channel(c), a.type, s_slab[i * S::SLAB + c] * inv);
+                if (a.lse && lane == 0)
+                    a.lse[(long long)tok * a.n_q_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945f;
+            }
+        }
+        named_bar_sync(1, 32 * KD_WARPS);
+        cur += cnt;
+    }
+}
+
+}  // namespace fence
