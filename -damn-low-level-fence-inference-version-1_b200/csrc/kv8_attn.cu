@@ -1,6 +1,6 @@
 // kv8_attn.cu — fence_kv8_attention: causal grouped-query attention of a ragged batch over the paged
 // 8-bit cache.
-#include "kv8_decode.cuh"
+#include "kv8_prefill.cuh"
 
 namespace fence {
 
@@ -49,13 +49,50 @@ static int kv8_launch_decode(const KAttnArgs& p, cudaStream_t st) {
     return cuda_status(cudaGetLastError(), "kv8_attention");
 }
 
+template <int FMT, int HD, bool SPLIT>
+static int kv8_launch_prefill(const KAttnArgs& p, cudaStream_t st) {
+    using S = KPShape<HD, SPLIT>;
+    static int done[64] = {};
+    CUtensorMap tm_k, tm_v;
+    const int box = p.c.page_tokens < 64 ? p.c.page_tokens : 64;
+    if (!kv8_tensor_map(&tm_k, &p.c, p.c.k, box) || !kv8_tensor_map(&tm_v, &p.c, p.c.v, box))
+        return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the cache");
+    auto kern = kv8_prefill_kernel<FMT, HD, SPLIT>;
+    FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM, done));
+    kern<<<KP_SMS, KP_THREADS, S::SMEM, st>>>(p, tm_k, tm_v);
+    return cuda_status(cudaGetLastError(), "kv8_attention");
+}
+
+constexpr size_t KV8_ARRIVED_BYTES = 4096;  // counters, at the workspace's start: 2048 for each kernel
+constexpr int KV8_DECODE_ROWS = 16;         // the most query rows per KV head of a request that the decode kernel takes in one pass
+
+// Whether the batch needs the prefill kernel.
+static bool kv8_has_prefill(const fence_kv8_cache* c, const fence_kv8_attn* a) {
+    return c->head_dim <= 128 && (long long)a->max_new * (a->n_q_heads / c->n_kv_heads) > KV8_DECODE_ROWS;
+}
+static size_t kv8_decode_part_bytes(const fence_kv8_cache* c) {
+    return (size_t)KV8_SMS * 2 * 2 * 16 * (c->head_dim + 2) * sizeof(float);
+}
+
 template <int FMT, int HD>
-static int kv8_launch_attn(const KAttnArgs& p, bool split, int nt, cudaStream_t st) {
+static int kv8_launch_attn(const KAttnArgs& pd, bool split, int nt, bool prefill, char* ws, cudaStream_t st) {
+    KAttnArgs p = pd;
+    if constexpr (HD <= 128) {
+        if (prefill) {
+            // one request: the prefill kernel takes it whatever its length is
+            p.min_rows = p.n_req == 1 ? 0 : KV8_DECODE_ROWS;
+            p.arrived = reinterpret_cast<int*>(ws + 2048);
+            p.part = reinterpret_cast<float*>(ws + KV8_ARRIVED_BYTES + kv8_decode_part_bytes(&p.c));
+            const int e = split ? kv8_launch_prefill<FMT, HD, true>(p, st) : kv8_launch_prefill<FMT, HD, false>(p, st);
+            if (e || p.n_req == 1) return e;
+            p.max_rows = KV8_DECODE_ROWS;
+            p.arrived = pd.arrived;
+            p.part = pd.part;
+        }
+    }
     if (split) return nt == 1 ? kv8_launch_decode<FMT, HD, true, 1>(p, st) : kv8_launch_decode<FMT, HD, true, 2>(p, st);
     return nt == 1 ? kv8_launch_decode<FMT, HD, false, 1>(p, st) : kv8_launch_decode<FMT, HD, false, 2>(p, st);
 }
-
-constexpr size_t KV8_ARRIVED_BYTES = 4096;  // counters, at the workspace's start
 
 static int kv8_attn_check(const fence_kv8_cache* c, const fence_paged_batch* b, const fence_kv8_attn* a, const char* who) {
     if (int e = kv8_check_cache(c, who)) return e;
@@ -64,6 +101,7 @@ static int kv8_attn_check(const fence_kv8_cache* c, const fence_paged_batch* b, 
     if (a->n_q_heads <= 0 || a->n_q_heads % c->n_kv_heads)
         return set_error(FENCE_E_ARG, "%s: %d query heads over %d kv heads", who, a->n_q_heads, c->n_kv_heads);
     if (!kv8_type_ok(a->type)) return set_error(FENCE_E_UNSUPPORTED, "%s: element type %d", who, a->type);
+    if (!(a->scale >= 0.f && a->scale < INFINITY)) return set_error(FENCE_E_ARG, "%s: scale %g", who, (double)a->scale);
     if (a->max_new <= 0) return set_error(FENCE_E_ARG, "%s: max_new %d", who, a->max_new);
     return FENCE_OK;
 }
@@ -74,7 +112,9 @@ extern "C" size_t fence_kv8_attention_workspace_bytes(const fence_kv8_cache* c, 
                                                       const fence_kv8_attn* a) {
     using namespace fence;
     if (kv8_attn_check(c, b, a, "kv8_attention_workspace_bytes")) return 0;
-    return KV8_ARRIVED_BYTES + (size_t)KV8_SMS * 2 * 2 * 16 * (c->head_dim + 2) * sizeof(float);
+    size_t n = KV8_ARRIVED_BYTES + kv8_decode_part_bytes(c);
+    if (kv8_has_prefill(c, a)) n += (size_t)KP_SMS * 4 * 128 * (c->head_dim + 2) * sizeof(float);
+    return n;
 }
 
 extern "C" int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_batch* b, const fence_kv8_attn* a,
@@ -97,18 +137,19 @@ extern "C" int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_b
         return set_error(FENCE_E_SCRATCH, "kv8_attention: workspace of %zu bytes, needs %zu", a->workspace_bytes, need);
     KAttnArgs p{*c, b->block_table, b->kv_len, b->new_start, b->n_req, b->n_tokens, b->max_pages, ilog2(c->page_tokens),
                 a->n_q_heads / c->n_kv_heads, a->n_q_heads, a->window > 0 ? a->window : 0, a->type, a->q, a->out, a->lse,
-                a->q_stride, a->out_stride, (float)(a->scale * 1.4426950408889634), INT_MAX, static_cast<int*>(a->workspace),
+                a->q_stride, a->out_stride, (float)(a->scale * 1.4426950408889634), INT_MAX, 0, kv8_wide(a->q, a->q_stride, a->type),
+                kv8_wide(a->out, a->out_stride, a->type), static_cast<int*>(a->workspace),
                 reinterpret_cast<float*>(static_cast<char*>(a->workspace) + KV8_ARRIVED_BYTES)};
-    const bool split = a->type == FENCE_F32;
+    const bool split = a->type == FENCE_F32, prefill = kv8_has_prefill(c, a);
     const int nt = (long long)a->max_new * p.G <= 8 ? 1 : 2;
     const cudaStream_t st = (cudaStream_t)stream;
     const int kind = (c->format == KV8_E4M3 ? 3 : 0) + (c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2);
     switch (kind) {
-        case 0: return kv8_launch_attn<KV8_INT8, 64>(p, split, nt, st);
-        case 1: return kv8_launch_attn<KV8_INT8, 128>(p, split, nt, st);
-        case 2: return kv8_launch_attn<KV8_INT8, 256>(p, split, nt, st);
-        case 3: return kv8_launch_attn<KV8_E4M3, 64>(p, split, nt, st);
-        case 4: return kv8_launch_attn<KV8_E4M3, 128>(p, split, nt, st);
-        default: return kv8_launch_attn<KV8_E4M3, 256>(p, split, nt, st);
+        case 0: return kv8_launch_attn<KV8_INT8, 64>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
+        case 1: return kv8_launch_attn<KV8_INT8, 128>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
+        case 2: return kv8_launch_attn<KV8_INT8, 256>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
+        case 3: return kv8_launch_attn<KV8_E4M3, 64>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
+        case 4: return kv8_launch_attn<KV8_E4M3, 128>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
+        default: return kv8_launch_attn<KV8_E4M3, 256>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
     }
 }

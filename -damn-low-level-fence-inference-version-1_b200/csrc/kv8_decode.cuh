@@ -38,7 +38,9 @@ struct KAttnArgs {
     float* lse;
     long long q_stride, out_stride;
     float scale_log2;  // scale * log2(e): scores are kept as exponents of 2
-    int max_rows;      // requests of more query rows per KV head are left to the other kernel
+    int max_rows;      // decode kernel: requests of more query rows per KV head are left to the prefill kernel
+    int min_rows;      // prefill kernel: requests of at most this many are the decode kernel's
+    int q_wide, out_wide;  // rows are 16-byte aligned
     int* arrived;      // [CTAs] partial results of the unit that starts in this CTA and goes on in the next
     float* part;       // [CTAs][2][rows * (head_dim + 2)]
 };
@@ -392,7 +394,8 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                 // ---- scale, mask, the largest of each row
                 const bool masked = !full_rows || key0 + 15 > lim_first || (a.window > 0 && key0 < all_lo);
                 float p[NT][4];
-                bool move = sv > vref;
+                const bool grow = sv > vref && sv < INFINITY;
+                bool move = grow;
                 float mt[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                 }
                 if (__any_sync(0xffffffffu, move)) {
                     float vf = 1.f;
-                    if (sv > vref) {
+                    if (grow) {
                         vinv = 1.f / sv;
                         vf = vref * vinv;
                         vref = sv;
@@ -438,7 +441,8 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                             }
                         }
                 }
-                const float fv = vref > 0.f ? sv * vinv : sv == 0.f ? 1.f : sv;  // NaN stays NaN
+                // a NaN or infinite scale gives NaN to whoever sees the key
+                const float fv = !(sv < INFINITY) ? __uint_as_float(0x7fffffffu) : vref > 0.f ? sv * vinv : 1.f;
                 uint32_t b0[NT], b1[NT], c0[NT], c1[NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
@@ -447,7 +451,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                         const float mm = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
                         const float x = kd_exp2(p[nt][e] - mm);
                         l[nt][e & 1] += x;
-                        p[nt][e] = x * fv;
+                        p[nt][e] = masked && p[nt][e] == -INFINITY ? 0.f : x * fv;
                     }
                     const uint32_t h0 = kd_pack(p[nt][0], p[nt][1]), h1 = kd_pack(p[nt][2], p[nt][3]);
                     b0[nt] = kd_transpose(h0);

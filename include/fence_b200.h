@@ -500,7 +500,7 @@ typedef struct fence_kv8_attn {
     int max_new;                   /* the most new tokens that a request brings (a hint for the
                                       choice of kernel: results do not depend on it beyond rounding) */
     int window;                    /* > 0: a query sees the last `window` positions only          */
-    float scale;                   /* of the scores, e.g. 1 / sqrt(head_dim)                     */
+    float scale;                   /* of the scores, e.g. 1 / sqrt(head_dim); finite, >= 0        */
     void* workspace;               /* fence_kv8_attention_workspace_bytes, 256-byte aligned; zeroed once
                                       by the caller before its first use, left ready by every call  */
     size_t workspace_bytes;

@@ -76,7 +76,8 @@ def test_store_and_load_refuse(fb, args):
 @pytest.mark.parametrize("field,value,code,text", [
     ("q", None, -1, "null"), ("workspace", None, -1, "null"), ("workspace", OK + 16, -2, "256-byte"), ("workspace_bytes", 8, -8, "needs"),
     ("n_q_heads", 7, -1, "query heads"), ("type", 5, -4, "type"), ("q_stride", 1023, -1, "strides"), ("out_stride", 1000, -1, "strides"),
-    ("max_new", 0, -1, "max_new"), ("q", OK + 2, -2, "aligned")])
+    ("max_new", 0, -1, "max_new"), ("scale", -0.5, -1, "scale"),
+    ("scale", float("nan"), -1, "scale"), ("scale", float("inf"), -1, "scale"), ("q", OK + 2, -2, "aligned")])
 def test_attention_refuses(fb, args, field, value, code, text):
     c, b, a = args
     setattr(a, field, value)
