@@ -53,13 +53,9 @@ template <int FMT, int HD, bool SPLIT>
 static int kv8_launch_prefill(const KAttnArgs& p, cudaStream_t st) {
     using S = KPShape<HD, SPLIT>;
     static int done[64] = {};
-    CUtensorMap tm_k, tm_v;
-    const int box = p.c.page_tokens < 64 ? p.c.page_tokens : 64;
-    if (!kv8_tensor_map(&tm_k, &p.c, p.c.k, box) || !kv8_tensor_map(&tm_v, &p.c, p.c.v, box))
-        return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the cache");
     auto kern = kv8_prefill_kernel<FMT, HD, SPLIT>;
     FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM, done));
-    kern<<<KP_SMS, KP_THREADS, S::SMEM, st>>>(p, tm_k, tm_v);
+    kern<<<KP_SMS, KP_THREADS, S::SMEM, st>>>(p);
     return cuda_status(cudaGetLastError(), "kv8_attention");
 }
 
@@ -153,3 +149,4 @@ extern "C" int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_b
         default: return kv8_launch_attn<KV8_E4M3, 256>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
     }
 }
+

@@ -13,46 +13,47 @@
 //    Two streams of 128 rows per CTA take turns on the matrix unit: while one stream's softmax warps
 //    work, the other's products run. fp32 activations (SPLIT): one group of 128 rows, q and the weights as
 //    pairs of fp16, and the two streams take the even and the odd tiles.
-//  * Codes become fp16 exactly, once per tile for both streams, by four converter warps: K rows as they
-//    are, V transposed, so that both are K-major operands in 128-byte swizzled shared memory. Scales never
-//    touch the codes: k_scale is part of a score's factor and v_scale / (a running reference) of the
-//    exponent, both constant over 16 keys.
+//  * Codes become fp16 exactly, once per tile for both streams, by four converter warps that fetch them a
+//    tile ahead (cp.async, a thread its own pieces) and store them as they lie, keys by channels, in 128-byte swizzled shared
+//    memory: a K-major operand for S, an MN-major one for O. Scales never touch the codes: k_scale is
+//    part of a score's factor and v_scale / (a running reference) of the exponent, both constant over 16 keys.
 //  * S, then P in its place as fp16 (the weights are the A operand straight from tensor memory), and O
 //    stay in tensor memory: 2 x (128 + head_dim) of its 512 columns.
 //  * O is rescaled only when a row's maximum grows by more than 2^8 (fp16 weights have that room).
 #pragma once
+
+#include <type_traits>
 
 #include "kv8_decode.cuh"
 
 namespace fence {
 
 constexpr int KP_KT = 128, KP_SMS = 148;
-constexpr int KP_W_CONV = 8, KP_W_LOAD = 12, KP_W_MMA = 13, KP_THREADS = 14 * 32;
-constexpr int KP_MIN_TILES = 2;
+constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_THREADS = 512;
+constexpr int KP_MIN_TILES = 2, KP_SLOTS = 4;
 
 template <int HD, bool SPLIT>
 struct KPShape {
     static constexpr int ROWS = SPLIT ? 128 : 256;  // per group
     static constexpr int Q_TILE = 128 * HD * 2;     // 128 rows as fp16
     static constexpr int OP = KP_KT * HD * 2;       // a K or V operand tile
-    static constexpr int RAW = KP_KT * HD;
     static constexpr int O_Q = 0;  // two tiles: the streams' rows, or the high and low parts
     static constexpr int O_K = 2 * Q_TILE;
     static constexpr int O_V = O_K + 2 * OP;
-    static constexpr int O_RK = O_V + 2 * OP;
-    static constexpr int O_RV = O_RK + RAW;
-    static constexpr int O_BAR = O_RV + RAW;
+    static constexpr int RAW = KP_KT * HD;          // staged codes of a K or V tile
+    static constexpr int O_RAW = O_V + 2 * OP;
+    static constexpr int O_BAR = O_RAW + 2 * RAW;
     static constexpr int O_MISC = O_BAR + 256;
-    static constexpr int O_RSC = O_MISC + 64;    // raw scales K 8, V 8
-    static constexpr int O_PREP = O_RSC + 64;    // [4][24]: k_scale, log2 v_scale, 1 / v_scale of 8 x 16 keys
-    static constexpr int SMEM = O_PREP + 4 * 96 + 1024;
-    static constexpr int REC = 128 * (HD + 2);   // floats of one stream's partial result
+    static constexpr int O_PREP = O_MISC + 64;  // [KP_SLOTS][32]: k_scale, log2 v_scale, 1 / v_scale, first row of 8 x 16 keys
+    static constexpr int SMEM = O_PREP + KP_SLOTS * 128 + 1024;
+    static constexpr int REC = 128 * (HD + 2);  // floats of one stream's partial result
 };
 
 // What every role derives for itself from the run's position.
 struct KPSeg {
     KReq q;
     int h, row0, nrows, tile0, cnt, first, tiles;  // this CTA's tiles of the unit, its place in the unit, the unit's tiles
+    int lo[2], hi[2];                              // the tiles that rows of each stream see
 };
 
 __device__ __forceinline__ void kp_group(const KAttnArgs& a, const KReq& q, int rows_per_group, int gi, int* lo_tile, int* tiles) {
@@ -134,45 +135,47 @@ struct KPWalk {
         s.tiles = t;
         s.tile0 = lo + rest;
         s.cnt = min(t - rest, end - cur);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int r_lo = s.row0 + (ROWS == 256 ? 128 * x : 0), r_hi = min(r_lo + 128, s.row0 + s.nrows) - 1;
+            const int first = q.kv - q.n + r_lo / a.G, last = q.kv - q.n + r_hi / a.G;
+            s.lo[x] = a.window > 0 ? max(0, first - a.window + 1) / KP_KT : 0;
+            s.hi[x] = r_hi < r_lo || last < 0 ? -1 : last / KP_KT;
+        }
         return s;
     }
 };
 
 // Whether stream s has rows that see the tile of keys kt.
 template <bool SPLIT>
-__device__ __forceinline__ bool kp_active(const KAttnArgs& a, const KPSeg& g, int s, int kt) {
-    if (SPLIT && (kt & 1) != s) return false;
-    const int r_lo = g.row0 + (SPLIT ? 0 : 128 * s), r_hi = min(r_lo + 128, g.row0 + g.nrows) - 1;
-    if (r_hi < r_lo) return false;
-    const int first = g.q.kv - g.q.n + r_lo / a.G, last = g.q.kv - g.q.n + r_hi / a.G;
-    const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-    return last >= 0 && kt * KP_KT <= last && (kt + 1) * KP_KT > lo;
+__device__ __forceinline__ bool kp_active(const KPSeg& g, int s, int kt) {
+    return kt >= g.lo[s] && kt <= g.hi[s] && (!SPLIT || (kt & 1) == s);
 }
 
 #define KP_LD32(r, addr)                                                                                                     \
     asm volatile(                                                                                                            \
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"             \
         "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"                                                   \
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),        \
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),             \
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),            \
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])                          \
+        : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7]),    \
+          "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]), "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]),             \
+          "=r"((r)[15]), "=r"((r)[16]), "=r"((r)[17]), "=r"((r)[18]), "=r"((r)[19]), "=r"((r)[20]), "=r"((r)[21]),           \
+          "=r"((r)[22]), "=r"((r)[23]), "=r"((r)[24]), "=r"((r)[25]), "=r"((r)[26]), "=r"((r)[27]), "=r"((r)[28]),           \
+          "=r"((r)[29]), "=r"((r)[30]), "=r"((r)[31])                                                                        \
         : "r"(addr)                                                                                                          \
         : "memory")
-#define KP_ST32(addr, r)                                                                                                     \
+#define KP_LD16(r, addr)                                                                                                     \
     asm volatile(                                                                                                            \
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"          \
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),                                         \
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),        \
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),          \
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),          \
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])                                                                       \
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"             \
+        : "=r"((r)[0]), "=r"((r)[1]), "=r"((r)[2]), "=r"((r)[3]), "=r"((r)[4]), "=r"((r)[5]), "=r"((r)[6]), "=r"((r)[7]),    \
+          "=r"((r)[8]), "=r"((r)[9]), "=r"((r)[10]), "=r"((r)[11]), "=r"((r)[12]), "=r"((r)[13]), "=r"((r)[14]),             \
+          "=r"((r)[15])                                                                                                      \
+        : "r"(addr)                                                                                                          \
         : "memory")
 #define KP_ST16(addr, r)                                                                                                     \
     asm volatile(                                                                                                            \
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), \
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),        \
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])                                               \
+        "r"((r)[0]), "r"((r)[1]), "r"((r)[2]), "r"((r)[3]), "r"((r)[4]), "r"((r)[5]), "r"((r)[6]), "r"((r)[7]), "r"((r)[8]),        \
+        "r"((r)[9]), "r"((r)[10]), "r"((r)[11]), "r"((r)[12]), "r"((r)[13]), "r"((r)[14]), "r"((r)[15])                       \
         : "memory")
 
 __device__ __forceinline__ void kp_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -199,8 +202,35 @@ __device__ __forceinline__ void kp_mma_ts(uint32_t d, uint32_t ta, uint64_t db, 
         "r"(ta), "l"(db), "r"(idesc), "r"((uint32_t)add)
         : "memory");
 }
-__device__ __forceinline__ void kp_sts32(uint32_t sa, uint32_t v) {
-    asm volatile("st.shared.b32 [%0], %1;" ::"r"(sa), "r"(v) : "memory");
+__device__ __forceinline__ void kp_sts64(uint32_t sa, uint32_t a, uint32_t b) {
+    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(sa), "r"(a), "r"(b) : "memory");
+}
+// two fp32 at once
+__device__ __forceinline__ uint64_t kp_two(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 kp_both(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t kp_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t kp_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// shared-memory descriptor of an MN-major operand, 128-byte swizzle: 8 keys of 128 bytes after 8 keys
+// (stride offset 1024), 64 channels after 64 channels (leading offset)
+__device__ __forceinline__ uint64_t kp_desc_mn(uint32_t saddr, uint32_t lead) {
+    return (uint64_t)((saddr >> 4) & 0x3FFFu) | ((uint64_t)(lead >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
 }
 __device__ __forceinline__ void kp_sts128(uint32_t sa, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sa), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -208,19 +238,17 @@ __device__ __forceinline__ void kp_sts128(uint32_t sa, uint32_t a, uint32_t b, u
 
 template <int FMT, int HD, bool SPLIT>
 __global__ void __launch_bounds__(KP_THREADS, 1)
-    kv8_prefill_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    kv8_prefill_kernel(const KAttnArgs a) {
     using S = KPShape<HD, SPLIT>;
-    constexpr int ROWS = S::ROWS, LINE = HD == 64 ? 64 : 128;
+    constexpr int ROWS = S::ROWS;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + S::O_BAR);
-    uint64_t *q_full = bar, *rk_full = bar + 2, *rk_empty = bar + 3, *rv_full = bar + 4, *rv_empty = bar + 5, *k_full = bar + 6,
-             *k_empty = bar + 8, *v_full = bar + 10, *v_empty = bar + 12, *s_full = bar + 14, *p_full = bar + 16, *o_full = bar + 18,
-             *prep_full = bar + 19, *seg_done = bar + 23;
+    uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = bar + 4, *v_full = bar + 6, *v_empty = bar + 8, *s_full = bar + 10,
+             *p_full = bar + 12, *o_full = bar + 14, *seg_done = bar + 15, *prep_full = bar + 16, *prep_empty = prep_full + KP_SLOTS;
     int* s_misc = reinterpret_cast<int*>(smem + S::O_MISC);
-    float* s_rsc = reinterpret_cast<float*>(smem + S::O_RSC);
     float* s_prep = reinterpret_cast<float*>(smem + S::O_PREP);
 
     if (tid == 0) {
@@ -233,13 +261,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 4);
         }
-        mbar_init(rk_full, 33);
-        mbar_init(rk_empty, 4);
-        mbar_init(rv_full, 1);
-        mbar_init(rv_empty, 4);
         mbar_init(o_full, 1);
         mbar_init(seg_done, 8);
-        for (int s = 0; s < 4; ++s) mbar_init(&prep_full[s], 1);
+        for (int s = 0; s < KP_SLOTS; ++s) {
+            mbar_init(&prep_full[s], 1);
+            mbar_init(&prep_empty[s], 12);
+        }
         fence_barrier_init();
     }
     if (warp == KP_W_MMA) {
@@ -319,172 +346,123 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         if (ok) ok = mbar_wait(b, n & 1u);
     };
 
-    if (warp == KP_W_LOAD) {
-        // ---------------------------------------------------------------- raw tiles and scales
-        const int P = a.c.page_tokens, box = min(P, 64), boxes = KP_KT / box;
+    if (warp >= KP_W_CONV && warp < KP_W_PREP) {
+        // ---------------------------------------------------------------- codes -> fp16 operands
+        // 8 keys x 64 channels a warp and step; rows r and r ^ 5 side by side: the stores of a quarter-warp do not meet on a bank.
+        // Items are K, V, K, V, ... of the tiles. A thread copies its own 16-byte pieces two items ahead and reads them back.
+        constexpr int HALF = HD / 64, STEPS = KP_KT / 8 * HALF / 4;
+        const int cw = warp - KP_W_CONV, r8 = (lane >> 3) ^ ((lane >> 2 & 1) * 5), P = a.c.page_tokens;
+        const uint32_t stage = sbase + S::O_RAW + (cw * 32 + lane) * 16;
+        uint32_t it = 0;
+        for (int cur = begin; cur < end;) {
+            const KPSeg g = walk.seek(a, cur, end);
+            const int any_lo = a.window > 0 ? max(0, g.q.kv - g.q.n + g.row0 / a.G - a.window + 1) : 0;
+            // the tiles that some row sees follow one another
+            const int t0 = max(g.tile0, min(g.hi[0] < 0 ? INT_MAX : g.lo[0], g.hi[1] < 0 ? INT_MAX : g.lo[1]));
+            const int t1 = min(g.tile0 + g.cnt - 1, max(g.hi[0], g.hi[1]));
+            const int n_items = 2 * max(0, t1 - t0 + 1);
+            for (int n = -2; n < n_items; ++n) {
+                const uint32_t t = it + (uint32_t)(n >> 1), b = t & 1u;  // the tile's count
+                const int v = n & 1;
+                if (n >= 0) {
+                    cp_async_wait_group<1>();
+                    if (t >= 2) wait((v ? v_empty : k_empty) + b, (t >> 1) - 1);
+                    __syncwarp();
+                    const uint32_t op = sbase + (v ? S::O_V : S::O_K) + b * S::OP, raw = stage + v * S::RAW;
+#pragma unroll 2
+                    for (int i = 0; i < STEPS; ++i) {
+                        const int row = ((i * 4 + cw) / HALF) * 8 + r8, half = (i * 4 + cw) % HALF;
+                        const uint4 x = lds128(raw + i * 2048);
+                        const uint32_t y[4] = {kd_bias<FMT>(x.x), kd_bias<FMT>(x.y), kd_bias<FMT>(x.z), kd_bias<FMT>(x.w)};
+                        const uint32_t dst = op + (uint32_t)(half * (KP_KT * 128) + row * 128);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            kp_sts128(dst + (((2 * (lane & 3) + k) ^ r8) << 4), kd_half2<FMT>(y[2 * k], false),
+                                      kd_half2<FMT>(y[2 * k], true), kd_half2<FMT>(y[2 * k + 1], false), kd_half2<FMT>(y[2 * k + 1], true));
+                    }
+                    kp_fence_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive((v ? v_full : k_full) + b);
+                }
+                if (n + 2 < n_items) {
+                    const uint32_t slot = (t + 1) % KP_SLOTS;
+                    const int key0 = (t0 + ((n + 2) >> 1)) * KP_KT;
+                    if (!v) wait(&prep_full[slot], (t + 1) / KP_SLOTS);
+                    const int* first = reinterpret_cast<const int*>(s_prep + slot * 32 + 24);
+                    const uint8_t* codes = static_cast<const uint8_t*>(v ? a.c.v : a.c.k);
+#pragma unroll 2
+                    for (int i = 0; i < STEPS; ++i) {
+                        const int row = ((i * 4 + cw) / HALF) * 8 + r8, half = (i * 4 + cw) % HALF, key = key0 + row;
+                        const bool in = key < g.q.kv && key >= any_lo;  // keys that no row sees may hold anything: they count as zero
+                        const uint8_t* src = codes + ((long long)first[row >> 4] * P + (key & (P - 1))) * HD + half * 64 + (lane & 3) * 16;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + v * S::RAW + i * 2048), "l"(src),
+                                     "r"(in ? 16 : 0)
+                                     : "memory");
+                    }
+                    __syncwarp();
+                    if (v && lane == 0) mbar_arrive(&prep_empty[slot]);
+                }
+                cp_async_commit();
+            }
+            it += (uint32_t)(n_items / 2);
+            cur += g.cnt;
+        }
+        cp_async_wait_all();
+    } else if (warp == KP_W_PREP) {
+        // ---------------------------------------------------------------- pages and scales of 8 x 16 keys, some tiles ahead
         uint32_t it = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
             const int* table = a.block_table + (size_t)walk.r * a.max_pages;
             for (int j = 0; j < g.cnt; ++j) {
-                const int kt = g.tile0 + j, key0 = kt * KP_KT;
-                if (!kp_active<SPLIT>(a, g, 0, kt) && !kp_active<SPLIT>(a, g, 1, kt)) continue;
-                // page of the 16 keys of lanes 0..7 (scales) and of this lane's box
-                auto page_at = [&](int key) {
+                const int kt = g.tile0 + j, key = kt * KP_KT + lane * 16;
+                if (!kp_active<SPLIT>(g, 0, kt) && !kp_active<SPLIT>(g, 1, kt)) continue;
+                int unit = 0;
+                float ks = 0.f, vs = 0.f;
+                if (lane < 8 && key < g.q.kv) {
                     int p = table[key >> a.shift];
                     if (p < 0 || p >= a.c.n_pages) {
                         set_device_error(KV8_BAD);
                         p = 0;
                     }
-                    return p * a.c.n_kv_heads + g.h;
-                };
-                const int k_box = key0 + lane * box, k_sc = key0 + lane * 16;
-                const bool load = lane < boxes && k_box < g.q.kv, scale = lane < 8 && k_sc < g.q.kv;
-                const int u_box = load ? page_at(k_box) : 0, u_sc = scale ? page_at(k_sc) : 0;
-                const int n = __popc(__ballot_sync(0xffffffffu, load));
-                if (it > 0) wait(rk_empty, it - 1);
-                if (!__all_sync(0xffffffffu, ok)) ok = false;
-                if (ok) {
-                    if (lane == 0) mbar_arrive_expect_tx(rk_full, (uint32_t)(n * box * HD));
-                    __syncwarp();
-                    if (load) kd_tma(sbase + S::O_RK + lane * box * LINE, &tm_k, 0, u_box * P + (k_box & (P - 1)), rk_full);
-                    if (scale) {
-                        cp_async4(s_rsc + lane, a.c.k_scale + u_sc);
-                        cp_async4(s_rsc + 8 + lane, a.c.v_scale + u_sc);
-                    }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(rk_full)) : "memory");
+                    unit = p * a.c.n_kv_heads + g.h;
+                    ks = a.c.k_scale[unit];
+                    vs = a.c.v_scale[unit];
                 }
-                if (it > 0) wait(rv_empty, it - 1);
-                if (!__all_sync(0xffffffffu, ok)) ok = false;
-                if (ok) {
-                    if (lane == 0) mbar_arrive_expect_tx(rv_full, (uint32_t)(n * box * HD));
-                    __syncwarp();
-                    if (load) kd_tma(sbase + S::O_RV + lane * box * LINE, &tm_v, 0, u_box * P + (k_box & (P - 1)), rv_full);
-                }
-                ++it;
-            }
-            cur += g.cnt;
-        }
-        cp_async_wait_all();
-    } else if (warp >= KP_W_CONV && warp < KP_W_LOAD) {
-        // ---------------------------------------------------------------- codes -> fp16 operands
-        const int cw = warp - KP_W_CONV;
-        uint32_t it = 0;
-        for (int cur = begin; cur < end;) {
-            const KPSeg g = walk.seek(a, cur, end);
-            const int any_lo = a.window > 0 ? max(0, g.q.kv - g.q.n + g.row0 / a.G - a.window + 1) : 0;
-            for (int j = 0; j < g.cnt; ++j) {
-                const int kt = g.tile0 + j, key0 = kt * KP_KT;
-                if (!kp_active<SPLIT>(a, g, 0, kt) && !kp_active<SPLIT>(a, g, 1, kt)) continue;
-                const uint32_t b = it & 1u;
-                // ---- K: rows as they are; a thread turns 16 codes into two 16-byte chunks
-                wait(rk_full, it);
-                if (it >= 2) wait(&k_empty[b], (it >> 1) - 1);
+                const uint32_t slot = it % KP_SLOTS;
+                if (it >= KP_SLOTS) wait(&prep_empty[slot], it / KP_SLOTS - 1);
                 __syncwarp();
-                if (cw == 0) {
-                    if (lane < 8) {
-                        const bool in = key0 + lane * 16 < g.q.kv;
-                        float ks = in ? s_rsc[lane] : 0.f;
-                        const float vs = in ? s_rsc[8 + lane] : 0.f;
-                        float lv = -INFINITY, rv = 1.f;
-                        if (vs > 0.f && vs < INFINITY) {
-                            lv = log2f(vs);
-                            rv = 1.f / vs;
-                        } else if (vs != 0.f) {
-                            ks = __uint_as_float(0x7fffffffu);  // NaN for whoever sees these keys
-                        }
-                        float* d = s_prep + (it & 3u) * 24;
-                        d[lane] = ks;
-                        d[8 + lane] = lv;
-                        d[16 + lane] = rv;
+                if (lane < 8) {
+                    float lv = -INFINITY, rv = 1.f;
+                    if (vs > 0.f && vs < INFINITY) {
+                        lv = log2f(vs);
+                        rv = 1.f / vs;
+                    } else if (vs != 0.f) {
+                        ks = __uint_as_float(0x7fffffffu);  // NaN for whoever sees these keys
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&prep_full[it & 3u]);
+                    float* d = s_prep + slot * 32;
+                    d[lane] = ks;
+                    d[8 + lane] = lv;
+                    d[16 + lane] = rv;
+                    reinterpret_cast<int*>(d)[24 + lane] = unit;
                 }
-                constexpr int CPR = HD / 16;  // 16-code chunks per row
-                const uint32_t kop = sbase + S::O_K + b * S::OP;
-#pragma unroll 4
-                for (int i = cw * 32 + lane; i < KP_KT * CPR; i += 128) {
-                    const int row = i / CPR, c = i % CPR;
-                    const uint32_t src = HD == 64 ? (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
-                                                  : (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4));
-                    const uint4 w = lds128(sbase + S::O_RK + src);
-                    const uint32_t x[4] = {kd_bias<FMT>(w.x), kd_bias<FMT>(w.y), kd_bias<FMT>(w.z), kd_bias<FMT>(w.w)};
-                    uint32_t y[8];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        y[2 * k] = kd_half2<FMT>(x[k], false);
-                        y[2 * k + 1] = kd_half2<FMT>(x[k], true);
-                    }
-                    const uint32_t dst = kop + (uint32_t)((c >> 2) * (KP_KT * 128) + row * 128);
-                    const uint32_t c0 = (uint32_t)((2 * c) & 7), f = (uint32_t)(row & 7);
-                    // the second slab's lanes store their chunks the other way round: no two on one bank
-                    const bool sw = HD == 128 && (c >> 2);
-                    const uint32_t ca = (c0 + (sw ? 1u : 0u)) ^ f, cb = (c0 + (sw ? 0u : 1u)) ^ f;
-                    kp_sts128(dst + (ca << 4), sw ? y[4] : y[0], sw ? y[5] : y[1], sw ? y[6] : y[2], sw ? y[7] : y[3]);
-                    kp_sts128(dst + (cb << 4), sw ? y[0] : y[4], sw ? y[1] : y[5], sw ? y[2] : y[6], sw ? y[3] : y[7]);
-                }
-                kp_fence_async();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(rk_empty);
-                    mbar_arrive(&k_full[b]);
-                }
-                // ---- V transposed: lanes are 32 pairs of keys, a thread turns 2 keys x 16 channels into 16 rows' words
-                wait(rv_full, it);
-                if (it >= 2) wait(&v_empty[b], (it >> 1) - 1);
-                __syncwarp();
-                const uint32_t vop = sbase + S::O_V + b * S::OP;
-                const bool edge = key0 + KP_KT > g.q.kv || key0 < any_lo;  // keys there may hold anything: they count as zero
-                const bool odd = (lane >> 2) & 1;  // these lanes read the odd key first: no two on one bank
-#pragma unroll 2
-                for (int i = cw; i < 2 * CPR; i += 4) {
-                    const int slab = i / CPR, c = i % CPR, row = slab * 64 + 2 * lane + (odd ? 1 : 0), row2 = row ^ 1;
-                    const uint32_t s1 = HD == 64 ? (uint32_t)(row * 64 + ((c ^ ((row >> 1) & 3)) << 4))
-                                                 : (uint32_t)(row * 128 + ((c ^ (row & 7)) << 4));
-                    const uint32_t s2 = HD == 64 ? (uint32_t)(row2 * 64 + ((c ^ ((row2 >> 1) & 3)) << 4))
-                                                 : (uint32_t)(row2 * 128 + ((c ^ (row2 & 7)) << 4));
-                    uint4 u = lds128(sbase + S::O_RV + s1), v = lds128(sbase + S::O_RV + s2);
-                    if (edge) {
-                        const int k1 = key0 + row, k2 = key0 + row2;
-                        if (k1 >= g.q.kv || k1 < any_lo) u = make_uint4(0, 0, 0, 0);
-                        if (k2 >= g.q.kv || k2 < any_lo) v = make_uint4(0, 0, 0, 0);
-                    }
-                    const uint32_t lo = odd ? 0x1504 : 0x5140, hi = odd ? 0x3726 : 0x7362;
-                    const uint32_t uu[4] = {u.x, u.y, u.z, u.w}, vv[4] = {v.x, v.y, v.z, v.w};
-                    const uint32_t dst = vop + (uint32_t)(slab * HD * 128 + c * 16 * 128 + (lane & 3) * 4);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t x = kd_bias<FMT>(__byte_perm(uu[k], vv[k], lo)), y = kd_bias<FMT>(__byte_perm(uu[k], vv[k], hi));
-                        const uint32_t w[4] = {kd_half2<FMT>(x, false), kd_half2<FMT>(x, true), kd_half2<FMT>(y, false),
-                                               kd_half2<FMT>(y, true)};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t d = 4 * k + e;  // channel 16 c + d: row of the operand, d & 7 its place in the swizzle
-                            kp_sts32(dst + d * 128 + ((((uint32_t)lane >> 2) ^ (d & 7u)) << 4), w[e]);
-                        }
-                    }
-                }
-                kp_fence_async();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(rv_empty);
-                    mbar_arrive(&v_full[b]);
-                }
+                if (lane == 0) mbar_arrive(&prep_full[slot]);
                 ++it;
             }
             cur += g.cnt;
         }
     } else if (warp == KP_W_MMA) {
         // ---------------------------------------------------------------- products
-        constexpr uint32_t id_s = tg_idesc(128, KP_KT), id_o = tg_idesc(128, HD);
+        constexpr uint32_t id_s = tg_idesc(128, KP_KT), id_o = tg_idesc(128, HD) | (1u << 16);  // V: MN-major
         uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0}, segs = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
             int pend[2] = {-1, -1};          // the tile (count) whose weights stream s is making
             bool have_q[2] = {false, false}, have_o[2] = {false, false};
-            int left[2] = {0, 0};            // streams that still need the V operand
-            auto weigh = [&](int s) {        // O_s += P_s . V of its pending tile
+            uint32_t left = 0;               // streams that still need the V operand: 8 bits per buffer
+            auto weigh = [&](auto stream) {  // O_s += P_s . V of its pending tile
+                constexpr int s = decltype(stream)::value;
                 const uint32_t t = (uint32_t)pend[s], b = t & 1u;
                 wait(&v_full[b], t >> 1);
                 wait(&p_full[s], np[s]++);
@@ -492,59 +470,66 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 kp_fence_after();
                 if (lane == 0 && ok) {
                     const uint32_t vop = sbase + S::O_V + b * S::OP;
-#pragma unroll
+#pragma unroll 1
                     for (int x = 0; x < (SPLIT ? 2 : 1); ++x) {
-#pragma unroll
+#pragma unroll 1
                         for (int k = 0; k < KP_KT / 16; ++k)
                             kp_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + (k >> 1) * 32 + x * 16 + (k & 1) * 8,
-                                      tg_desc(vop + (k >> 2) * HD * 128 + (k & 3) * 32), id_o, have_o[s] || x > 0 || k > 0);
+                                      kp_desc_mn(vop + k * 2048, KP_KT * 128), id_o, have_o[s] || x > 0 || k > 0);
                     }
                 }
                 have_o[s] = true;
-                if (--left[b] == 0 && lane == 0 && ok) kp_commit(&v_empty[b]);
+                left -= 1u << (8 * b);
+                if (((left >> (8 * b)) & 255u) == 0 && lane == 0 && ok) kp_commit(&v_empty[b]);
                 pend[s] = -1;
             };
+            auto score = [&](auto stream, uint32_t b) {  // S_s = Q_s . K^T
+                constexpr int s = decltype(stream)::value;
+                constexpr int qi = SPLIT ? 0 : s;
+                if (!have_q[qi]) {
+                    have_q[qi] = true;
+                    wait(&q_full[qi], nq[qi]++);
+                }
+                wait(&k_full[b], it >> 1);
+                __syncwarp();
+                kp_fence_after();
+                if (lane == 0 && ok) {
+                    const uint32_t kop = sbase + S::O_K + b * S::OP;
+#pragma unroll 1
+                    for (int x = SPLIT ? 1 : 0; x >= 0; --x) {  // the low parts first
+                        const uint32_t qop = sbase + S::O_Q + (SPLIT ? x : s) * S::Q_TILE;
+#pragma unroll 1
+                        for (int k = 0; k < HD / 16; ++k)
+                            kp_mma_ss(tmem + 128 * s, tg_desc(qop + (k >> 2) * 128 * 128 + (k & 3) * 32),
+                                      tg_desc(kop + (k >> 2) * KP_KT * 128 + (k & 3) * 32), id_s, (SPLIT && x == 0) || k > 0);
+                    }
+                    kp_commit(&s_full[s]);
+                }
+                pend[s] = (int)it;
+            };
+            constexpr std::integral_constant<int, 0> st0{};
+            constexpr std::integral_constant<int, 1> st1{};
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j;
-                const bool act[2] = {kp_active<SPLIT>(a, g, 0, kt), kp_active<SPLIT>(a, g, 1, kt)};
-                if (!act[0] && !act[1]) continue;
+                const bool act0 = kp_active<SPLIT>(g, 0, kt), act1 = kp_active<SPLIT>(g, 1, kt);
+                if (!act0 && !act1) continue;
                 const uint32_t b = it & 1u;
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    if (pend[s] >= 0 && (!SPLIT || act[s])) weigh(s);
-                    if (!act[s]) continue;
-                    if (!have_q[SPLIT ? 0 : s]) {
-                        have_q[SPLIT ? 0 : s] = true;
-                        wait(&q_full[SPLIT ? 0 : s], nq[SPLIT ? 0 : s]++);
-                    }
-                    wait(&k_full[b], it >> 1);
-                    __syncwarp();
-                    kp_fence_after();
-                    if (lane == 0 && ok) {
-                        const uint32_t kop = sbase + S::O_K + b * S::OP;
-#pragma unroll
-                        for (int x = SPLIT ? 1 : 0; x >= 0; --x) {  // the low parts first
-                            const uint32_t qop = sbase + S::O_Q + (SPLIT ? x : s) * S::Q_TILE;
-#pragma unroll
-                            for (int k = 0; k < HD / 16; ++k)
-                                kp_mma_ss(tmem + 128 * s, tg_desc(qop + (k >> 2) * 128 * 128 + (k & 3) * 32),
-                                          tg_desc(kop + (k >> 2) * KP_KT * 128 + (k & 3) * 32), id_s, (SPLIT && x == 0) || k > 0);
-                        }
-                        kp_commit(&s_full[s]);
-                    }
-                    pend[s] = (int)it;
-                }
-                left[b] = (act[0] ? 1 : 0) + (act[1] ? 1 : 0);
+                if (pend[0] >= 0 && (!SPLIT || act0)) weigh(st0);
+                if (act0) score(st0, b);
+                if (pend[1] >= 0 && (!SPLIT || act1)) weigh(st1);
+                if (act1) score(st1, b);
+                left += ((act0 ? 1u : 0u) + (act1 ? 1u : 0u)) << (8 * b);
                 if (lane == 0 && ok) kp_commit(&k_empty[b]);
                 ++it;
             }
             // the last tiles' weights, in the order of the tiles
-            const int s0 = pend[0] >= 0 && (pend[1] < 0 || pend[0] <= pend[1]) ? 0 : 1;
-            if (pend[s0] >= 0) weigh(s0);
-            if (pend[1 - s0] >= 0) weigh(1 - s0);
+            if (pend[0] >= 0 && (pend[1] < 0 || pend[0] <= pend[1])) weigh(st0);
+            if (pend[1] >= 0) weigh(st1);
+            if (pend[0] >= 0) weigh(st0);
             // a stream without tiles here may still be at the last unit's end: o_full must not run two ahead of it
             if (segs > 0) wait(seg_done, segs - 1);
             ++segs;
+            __syncwarp();
             if (lane == 0 && ok) kp_commit(o_full);
             __syncwarp();
             cur += g.cnt;
@@ -575,48 +560,91 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const int lim_lo = a.window > 0 ? lim - a.window + 1 : 0;
             // tiles that all of this stream's rows see whole need no mask
             const int r_lo = g.row0 + (SPLIT ? 0 : 128 * s), r_hi = min(r_lo + 128, g.row0 + g.nrows) - 1;
-            const bool rows_full = r_hi - r_lo == 127;
             const int lim_first = g.q.kv - g.q.n + r_lo / a.G, lim_last = g.q.kv - g.q.n + r_hi / a.G;
-            bool any = false;
-            for (int j = 0; j < g.cnt && !any; ++j) any = kp_active<SPLIT>(a, g, s, g.tile0 + j);
-            bool any_q = any;
-            if (SPLIT && s == 0)
-                for (int j = 0; j < g.cnt && !any_q; ++j) any_q = kp_active<SPLIT>(a, g, 1, g.tile0 + j);
+            // whether this stream's q operand is used here (SPLIT: the other stream's tiles use it too)
+            const bool any_q = max(g.lo[s], g.tile0) <= min(g.hi[s], g.tile0 + g.cnt - 1);
             float qs = 1.f;
             if (any_q) {
-                // ---- this row of q: by a power of two into [256, 512), fp16 (and what fp16 leaves)
+                // ---- q: rows by a power of two into [256, 512), fp16 (and what fp16 leaves); all lanes on one row at a time
+                constexpr int EPL = HD / 32, BATCH = 8;
                 const long long at = tok * a.q_stride + (long long)head * HD;
-                uint32_t big = 0;
-#pragma unroll 4
-                for (int c = 0; c < HD; c += 8) {
-                    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                    if (valid) kv8_ld8(a.q, at + c, a.type, a.q_wide, x);
+#pragma unroll 1
+                for (int r0 = 0; r0 < 32; r0 += BATCH) {
+                    uint32_t w[BATCH][SPLIT ? EPL : EPL / 2];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
-                }
-                const int ex = (int)(big >> 23);
-                const bool plain = ex == 255;
-                const int sh = plain ? 0 : max(ex, 1) - 127 - 8;
-                const float f1 = __uint_as_float((uint32_t)(127 - max(min(sh, 126), -126)) << 23);
-                const float f2 = sh < -126 ? __uint_as_float((uint32_t)(1 - sh) << 23) : 1.f;
-                qs = (plain ? 1.f : ldexpf(1.f, sh)) * a.scale_log2;
-                if (!SPLIT || s == 0) {
-                    const uint32_t dst = sbase + S::O_Q + (SPLIT ? 0 : s * S::Q_TILE) + row * 128;
-#pragma unroll 4
-                    for (int c = 0; c < HD; c += 8) {
-                        float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                        if (valid) kv8_ld8(a.q, at + c, a.type, a.q_wide, x);
-                        uint32_t hi[4], lo[4];
+                    for (int i = 0; i < BATCH; ++i) {
+                        const long long src = __shfl_sync(0xffffffffu, at, r0 + i) + lane * EPL;
+                        const bool in = __shfl_sync(0xffffffffu, (int)valid, r0 + i);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float u = x[2 * e] * f1 * f2, v = x[2 * e + 1] * f1 * f2;
-                            hi[e] = kd_pack(u, v);
-                            if (SPLIT) lo[e] = kd_pack_rest(u, v, hi[e]);
+                        for (int e = 0; e < (SPLIT ? EPL : EPL / 2); ++e) w[i][e] = 0;
+                        if (in) {
+                            if (SPLIT) {
+                                const uint32_t* p = static_cast<const uint32_t*>(a.q) + src;
+                                if (a.q_wide && EPL == 4) {
+                                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+                                    w[i][0] = v.x, w[i][1] = v.y, w[i][EPL - 2] = v.z, w[i][EPL - 1] = v.w;
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < EPL; ++e) w[i][e] = __ldg(p + e);
+                                }
+                            } else {
+                                const uint16_t* p = static_cast<const uint16_t*>(a.q) + src;
+                                if (a.q_wide && EPL == 4) {
+                                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
+                                    w[i][0] = v.x, w[i][EPL / 2 - 1] = v.y;
+                                } else {
+#pragma unroll
+                                    for (int e = 0; e < EPL / 2; ++e)
+                                        w[i][e] = (uint32_t)__ldg(p + 2 * e) | ((uint32_t)__ldg(p + 2 * e + 1) << 16);
+                                }
+                            }
                         }
-                        const uint32_t o = dst + (c >> 6) * (128 * 128) + ((((c >> 3) & 7) ^ (row & 7)) << 4);
-                        kp_sts128(o, hi[0], hi[1], hi[2], hi[3]);
-                        if (SPLIT) kp_sts128(o + S::Q_TILE, lo[0], lo[1], lo[2], lo[3]);
                     }
+#pragma unroll
+                    for (int i = 0; i < BATCH; ++i) {
+                        float x[EPL];
+#pragma unroll
+                        for (int e = 0; e < EPL; e += 2) {
+                            if (SPLIT) {
+                                x[e] = __uint_as_float(w[i][SPLIT ? e : 0]), x[e + 1] = __uint_as_float(w[i][SPLIT ? e + 1 : 0]);
+                            } else if (a.type == FENCE_F16) {
+                                x[e] = half_bits_to_float(w[i][e / 2]), x[e + 1] = half_bits_to_float(w[i][e / 2] >> 16);
+                            } else {
+                                x[e] = __uint_as_float(w[i][e / 2] << 16), x[e + 1] = __uint_as_float(w[i][e / 2] & 0xffff0000u);
+                            }
+                        }
+                        uint32_t big = 0;
+#pragma unroll
+                        for (int e = 0; e < EPL; ++e) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
+                        big = __reduce_max_sync(0xffffffffu, big);
+                        const int ex = (int)(big >> 23);
+                        const bool plain = ex == 255;
+                        const int sh = plain ? 0 : max(ex, 1) - 127 - 8;
+                        const float f1 = __uint_as_float((uint32_t)(127 - max(min(sh, 126), -126)) << 23);
+                        const float f2 = sh < -126 ? __uint_as_float((uint32_t)(1 - sh) << 23) : 1.f;
+                        if (lane == r0 + i) qs = (plain ? 1.f : ldexpf(1.f, sh)) * a.scale_log2;
+                        if (!SPLIT || s == 0) {
+                            const int qrow = (warp & 3) * 32 + r0 + i, c = lane * EPL;
+                            const uint32_t dst = sbase + S::O_Q + (SPLIT ? 0 : s * S::Q_TILE) + (c >> 6) * (128 * 128) + qrow * 128 +
+                                                 ((((c >> 3) & 7) ^ (qrow & 7)) << 4) + (c & 7) * 2;
+                            uint32_t hi[EPL / 2], lo[EPL / 2];
+#pragma unroll
+                            for (int e = 0; e < EPL; e += 2) {
+                                const float u = x[e] * f1 * f2, v = x[e + 1] * f1 * f2;
+                                hi[e / 2] = kd_pack(u, v);
+                                lo[e / 2] = SPLIT ? kd_pack_rest(u, v, hi[e / 2]) : 0u;
+                            }
+                            if (EPL == 4) {
+                                kp_sts64(dst, hi[0], hi[EPL / 2 - 1]);
+                                if (SPLIT) kp_sts64(dst + S::Q_TILE, lo[0], lo[EPL / 2 - 1]);
+                            } else {
+                                asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(hi[0]) : "memory");
+                                if (SPLIT) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + S::Q_TILE), "r"(lo[0]) : "memory");
+                            }
+                        }
+                    }
+                }
+                if (!SPLIT || s == 0) {
                     kp_fence_async();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&q_full[SPLIT ? 0 : s]);
@@ -626,39 +654,63 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             bool have_o = false;
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j, key0 = kt * KP_KT;
-                const bool act = kp_active<SPLIT>(a, g, s, kt);
-                if (!act && !kp_active<SPLIT>(a, g, 1 - s, kt)) continue;
-                const uint32_t slot = it & 3u, use = it >> 2;
+                const bool act = kp_active<SPLIT>(g, s, kt);
+                if (!act && !kp_active<SPLIT>(g, 1 - s, kt)) continue;
+                const uint32_t slot = it % KP_SLOTS, use = it / KP_SLOTS;
                 ++it;
-                if (!act) continue;
-                wait(&prep_full[slot], use);
+                wait(&prep_full[slot], use);  // also where this stream has no rows: it must not give back a slot before its time
+                __syncwarp();
+                if (!act) {
+                    if (lane == 0) mbar_arrive(&prep_empty[slot]);
+                    continue;
+                }
                 wait(&s_full[s], n_s++);
                 __syncwarp();
                 kp_fence_after();
-                const float* pr = s_prep + slot * 24;
-                const bool masked = !rows_full || key0 + KP_KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
-                const int c_hi = lim - key0, c_lo = lim_lo - key0;  // this row sees the columns c_lo .. c_hi
-                // ---- the row's largest
-                float mt = -INFINITY, lvmax = -INFINITY;
+                const float* pr = s_prep + slot * 32;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
+                // Loops of 32 columns, not unrolled: the roles' code has to share the instruction cache.
+                const bool edge = key0 + KP_KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
+                uint32_t bad = 0;  // of an edge tile: blocks of 16 keys with a scale that is no number, of which this row sees some
+                if (edge) {        // -infinity in the columns that this row does not see
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        KP_LD32(x, t_s + 32 * c);
+                        kp_wait_ld();
+                        const int h = lim - key0 - 32 * c, l0 = lim_lo - key0 - 32 * c;  // sees the columns l0 .. h
+                        uint32_t see = h < 0 ? 0u : h >= 31 ? ~0u : (2u << h) - 1u;
+                        if (l0 > 0) see &= l0 >= 32 ? 0u : ~0u << l0;
 #pragma unroll
-                for (int b = 0; b < 8; ++b) lvmax = fmaxf(lvmax, pr[8 + b]);
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32];
-                    KP_LD32(r, t_s + c * 32);
-                    kp_wait_ld();
-#pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        float x = -INFINITY;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const int col = c * 32 + b * 16 + e;
-                            float y = __uint_as_float(r[b * 16 + e]);
-                            if (masked && (col > c_hi || col < c_lo)) y = -INFINITY;
-                            x = fmaxf(x, y);
-                        }
-                        mt = fmaxf(mt, x * (pr[c * 2 + b] * qs));
+                        for (int e = 0; e < 32; ++e)
+                            if (!((see >> e) & 1u)) x[e] = 0xff800000u;
+                        KP_ST16(t_s + 32 * c, x);
+                        KP_ST16(t_s + 32 * c + 16, (x + 16));
+                        if (!(pr[2 * c] * qs < INFINITY) && (see & 0xffffu)) bad |= 1u << (2 * c);
+                        if (!(pr[2 * c + 1] * qs < INFINITY) && (see >> 16)) bad |= 2u << (2 * c);
                     }
+                    kp_wait_st();
+                }
+                // factor of a block's scores; -infinity has to stay so in an edge tile: none of 0 or NaN there
+                auto factor = [&](int b) {
+                    float f = pr[b] * qs;
+                    if (edge) f = f < INFINITY ? fmaxf(f, 1e-30f) : 1e-30f;
+                    return f;
+                };
+                float mt = -INFINITY, lvmax = -INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t x[32];
+                    KP_LD32(x, t_s + 32 * c);
+                    const float f0 = factor(2 * c), f1 = factor(2 * c + 1);
+                    lvmax = fmaxf(lvmax, fmaxf(pr[8 + 2 * c], pr[9 + 2 * c]));
+                    kp_wait_ld();
+                    float y0 = __uint_as_float(x[0]), y1 = __uint_as_float(x[16]);
+#pragma unroll
+                    for (int e = 1; e < 16; ++e) {
+                        y0 = fmaxf(y0, __uint_as_float(x[e]));
+                        y1 = fmaxf(y1, __uint_as_float(x[16 + e]));
+                    }
+                    mt = fmaxf(mt, fmaxf(y0 * f0, y1 * f1));
                 }
                 const bool move_v = lvmax > lvref + 4.f;
                 if (__any_sync(0xffffffffu, move_v || mt > m + KD_LAZY)) {
@@ -672,48 +724,54 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     }
                     m = mn;
                     if (have_o) {  // the products of the tiles before have ended: S came after them
-#pragma unroll
-                        for (int c = 0; c < HD; c += 32) {
-                            uint32_t r[32];
-                            KP_LD32(r, t_o + c);
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t r[16];
+                            KP_LD16(r, t_o + c);
                             kp_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * al);
-                            KP_ST32(t_o + c, r);
+                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * al);
+                            KP_ST16(t_o + c, r);
                         }
                     }
                 }
                 have_o = true;
                 const float mm = m == -INFINITY ? 0.f : m, lv0 = lvref == -INFINITY ? 0.f : lvref;
                 // ---- weights, in place of the scores
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 4; ++c) {
-                    uint32_t r[32], hi[16], lo[16];
-                    KP_LD32(r, t_s + c * 32);
+                    uint32_t x[32], hi[16], lo[16];
+                    KP_LD32(x, t_s + 32 * c);
+                    float cf[2], add[2], fb[2], fl[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int b = 2 * c + k;
+                        const float d = pr[8 + b] - lv0;
+                        const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it
+                        cf[k] = factor(b);
+                        add[k] = SPLIT ? -mm : (tiny ? -40.f : d) - mm;
+                        if ((bad >> b) & 1u) add[k] = __uint_as_float(0x7fffffffu);
+                        fb[k] = SPLIT ? (tiny ? 0.f : kd_exp2(d)) : 0.f;
+                        fl[k] = SPLIT ? 1.f : tiny ? 1.0995116e12f : pr[16 + b] * (lvref == -INFINITY ? 1.f : vref);
+                    }
                     kp_wait_ld();
 #pragma unroll
-                    for (int b = 0; b < 2; ++b) {
-                        const float cf = pr[c * 2 + b] * qs, d = pr[8 + c * 2 + b] - lv0;
-                        const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it
-                        const float add = SPLIT ? -mm : (tiny ? -40.f : d) - mm;
-                        const float fb = SPLIT ? (tiny ? 0.f : kd_exp2(d)) : 0.f;
-                        float sum = 0.f;
+                    for (int k = 0; k < 2; ++k) {
+                        const uint64_t cf2 = kp_two(cf[k], cf[k]), add2 = kp_two(add[k], add[k]);
+                        uint64_t sum2 = 0;
 #pragma unroll
                         for (int e = 0; e < 16; e += 2) {
-                            float p[2];
-#pragma unroll
-                            for (int y = 0; y < 2; ++y) {
-                                const int col = c * 32 + b * 16 + e + y;
-                                p[y] = kd_exp2(fmaf(__uint_as_float(r[b * 16 + e + y]), cf, add));
-                                if (masked && (col > c_hi || col < c_lo)) p[y] = 0.f;
-                                sum += p[y];
-                                if (SPLIT) p[y] *= fb;
-                            }
-                            const int at = b * 8 + (e >> 1);
-                            hi[at] = kd_pack(p[0], p[1]);
-                            if (SPLIT) lo[at] = kd_pack_rest(p[0], p[1], hi[at]);
+                            const float2 y = kp_both(
+                                kp_fma2(kp_two(__uint_as_float(x[16 * k + e]), __uint_as_float(x[16 * k + e + 1])), cf2, add2));
+                            float p0 = kd_exp2(y.x), p1 = kd_exp2(y.y);
+                            sum2 = kp_add2(sum2, kp_two(p0, p1));
+                            if (SPLIT) p0 *= fb[k], p1 *= fb[k];
+                            const int at = k * 8 + (e >> 1);
+                            hi[at] = kd_pack(p0, p1);
+                            if (SPLIT) lo[at] = kd_pack_rest(p0, p1, hi[at]);
                         }
-                        l += SPLIT ? sum : sum * (tiny ? 1.0995116e12f : pr[16 + c * 2 + b] * (lvref == -INFINITY ? 1.f : vref));
+                        const float2 sum = kp_both(sum2);
+                        l += (sum.x + sum.y) * fl[k];
                     }
                     KP_ST16(t_s + c * 32, hi);
                     if (SPLIT) KP_ST16(t_s + c * 32 + 16, lo);
@@ -721,7 +779,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 kp_wait_st();
                 kp_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[s]);
+                if (lane == 0) {
+                    mbar_arrive(&p_full[s]);
+                    mbar_arrive(&prep_empty[slot]);
+                }
             }
             // ---- the unit's (or this part's) end
             wait(o_full, n_o++);
@@ -730,46 +791,36 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const bool whole = g.cnt == g.tiles, direct = whole && !SPLIT;
             const int unit0 = cur - g.first;
             const int c_first = unit0 / per, c_last = (unit0 + g.tiles - 1) / per;
-            if (direct) {
-                const float inv = l == 0.f ? 0.f : vref / l;
-#pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t r[32];
-                    if (have_o) {
-                        KP_LD32(r, t_o + c);
-                        kp_wait_ld();
-                    }
-                    if (valid) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            float x[8];
-#pragma unroll
-                            for (int y = 0; y < 8; ++y) x[y] = have_o && l != 0.f ? __uint_as_float(r[e + y]) * inv : 0.f;
-                            kv8_st8(a.out, tok * a.out_stride + (long long)head * HD + c + e, a.type, a.out_wide, x);
-                        }
-                    }
+            // the sums go out as they are, or to the record of (CTA, slot, stream): m and l of each row, then four channels
+            // of all rows after one another
+            float* rec = a.part + ((long long)blockIdx.x * 4 + (g.first > 0 ? 0 : 2) + s) * S::REC;
+            const float mul = direct ? (l == 0.f ? 0.f : vref / l) : vref;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+                uint32_t r[16];
+                float x[16];
+                if (have_o) {
+                    KP_LD16(r, t_o + c);
+                    kp_wait_ld();
                 }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[e] = have_o && mul != 0.f ? __uint_as_float(r[e]) * mul : 0.f;
+                if (direct) {
+                    const long long at = tok * a.out_stride + (long long)head * HD + c;
+                    if (valid) {
+                        kv8_st8(a.out, at, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x));
+                        kv8_st8(a.out, at + 8, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x + 8));
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4)
+                        __stcg(reinterpret_cast<float4*>(rec + 256) + ((c + e) >> 2) * 128 + row, make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                }
+            }
+            if (direct) {
                 if (valid && a.lse) a.lse[tok * a.n_q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
             } else {
-                // record of (CTA, slot, stream): m and l of each row, then the sums, four channels of all rows after one another
-                float* rec = a.part + ((long long)blockIdx.x * 4 + (g.first > 0 ? 0 : 2) + s) * S::REC;
                 __stcg(reinterpret_cast<float2*>(rec) + row, make_float2(m, l));
-#pragma unroll
-                for (int c = 0; c < HD; c += 32) {
-                    uint32_t r[32];
-                    if (have_o) {
-                        KP_LD32(r, t_o + c);
-                        kp_wait_ld();
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (have_o)
-                            v = make_float4(__uint_as_float(r[e]) * vref, __uint_as_float(r[e + 1]) * vref,
-                                            __uint_as_float(r[e + 2]) * vref, __uint_as_float(r[e + 3]) * vref);
-                        __stcg(reinterpret_cast<float4*>(rec + 256) + ((c + e) >> 2) * 128 + row, v);
-                    }
-                }
                 __threadfence();
                 named_bar_sync(1, 256);
                 if (tid == 0) {
@@ -785,6 +836,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     constexpr int STREAMS = SPLIT ? 2 : 1;
                     const int c0 = SPLIT ? s * (HD / 2) : 0, c1 = SPLIT ? c0 + HD / 2 : HD;
                     float M = -INFINITY, L = 0.f;
+#pragma unroll 1
                     for (int k = c_first; k <= c_last; ++k)
 #pragma unroll
                         for (int x = 0; x < STREAMS; ++x) {
@@ -795,10 +847,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                             M = mn;
                         }
                     const float mz = M == -INFINITY ? 0.f : M, inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll 1
                     for (int c = c0; c < c1; c += 32) {
                         float acc[32];
 #pragma unroll
                         for (int e = 0; e < 32; ++e) acc[e] = 0.f;
+#pragma unroll 1
                         for (int k = c_first; k <= c_last; ++k)
 #pragma unroll
                             for (int x = 0; x < STREAMS; ++x) {
