@@ -53,9 +53,13 @@ template <int FMT, int HD, bool SPLIT>
 static int kv8_launch_prefill(const KAttnArgs& p, cudaStream_t st) {
     using S = KPShape<HD, SPLIT>;
     static int done[64] = {};
+    CUtensorMap tm_k, tm_v;
+    const int box = p.c.page_tokens < 64 ? p.c.page_tokens : 64;
+    if (!kv8_tensor_map(&tm_k, &p.c, p.c.k, box) || !kv8_tensor_map(&tm_v, &p.c, p.c.v, box))
+        return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the cache");
     auto kern = kv8_prefill_kernel<FMT, HD, SPLIT>;
     FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM, done));
-    kern<<<KP_SMS, KP_THREADS, S::SMEM, st>>>(p);
+    kern<<<KP_SMS, KP_THREADS, S::SMEM, st>>>(p, tm_k, tm_v);
     return cuda_status(cudaGetLastError(), "kv8_attention");
 }
 

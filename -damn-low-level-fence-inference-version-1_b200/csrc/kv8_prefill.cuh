@@ -13,8 +13,8 @@
 //    Two streams of 128 rows per CTA take turns on the matrix unit: while one stream's softmax warps
 //    work, the other's products run. fp32 activations (SPLIT): one group of 128 rows, q and the weights as
 //    pairs of fp16, and the two streams take the even and the odd tiles.
-//  * Codes become fp16 exactly, once per tile for both streams, by four converter warps that fetch them a
-//    tile ahead (cp.async, a thread its own pieces) and store them as they lie, keys by channels, in 128-byte swizzled shared
+//  * Codes become fp16 exactly, once per tile for both streams, by four converter warps, from stages that
+//    TMA fills a tile ahead, and stored as they lie, keys by channels, in 128-byte swizzled shared
 //    memory: a K-major operand for S, an MN-major one for O. Scales never touch the codes: k_scale is
 //    part of a score's factor and v_scale / (a running reference) of the exponent, both constant over 16 keys.
 //  * S, then P in its place as fp16 (the weights are the A operand straight from tensor memory), and O
@@ -29,7 +29,7 @@
 namespace fence {
 
 constexpr int KP_KT = 128, KP_SMS = 148;
-constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_THREADS = 512;
+constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_W_LOAD = 14, KP_THREADS = 480;
 constexpr int KP_MIN_TILES = 2, KP_SLOTS = 4;
 
 template <int HD, bool SPLIT>
@@ -44,7 +44,7 @@ struct KPShape {
     static constexpr int O_RAW = O_V + 2 * OP;
     static constexpr int O_BAR = O_RAW + 2 * RAW;
     static constexpr int O_MISC = O_BAR + 256;
-    static constexpr int O_PREP = O_MISC + 64;  // [KP_SLOTS][32]: k_scale, log2 v_scale, 1 / v_scale, first row of 8 x 16 keys
+    static constexpr int O_PREP = O_MISC + 64;  // [KP_SLOTS][24]: k_scale, log2 v_scale, 1 / v_scale of 8 x 16 keys; [KP_SLOTS][8]: the pool's row of their first
     static constexpr int SMEM = O_PREP + KP_SLOTS * 128 + 1024;
     static constexpr int REC = 128 * (HD + 2);  // floats of one stream's partial result
 };
@@ -184,22 +184,29 @@ __device__ __forceinline__ void kp_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void kp_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // what this thread wrote to shared memory is visible to the matrix unit's reads
 __device__ __forceinline__ void kp_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// One lane of the warp, always the same: the matrix unit's calls are made by it.
+__device__ __forceinline__ bool kp_elect() {
+    uint32_t e;
+    asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(e));
+    return e != 0;
+}
 __device__ __forceinline__ void kp_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // D (tensor memory) (+)= A (shared memory) . B^T, and the same with A in tensor memory
-__device__ __forceinline__ void kp_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool add) {
+template <bool ADD>
+__device__ __forceinline__ void kp_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)add)
+        "l"(da), "l"(db), "r"(idesc), "n"(ADD ? 1 : 0)
         : "memory");
 }
-__device__ __forceinline__ void kp_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, bool add) {
+__device__ __forceinline__ void kp_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(ta), "l"(db), "r"(idesc), "r"((uint32_t)add)
+        "r"(ta), "l"(db), "r"(idesc), "r"(add)
         : "memory");
 }
 __device__ __forceinline__ void kp_sts64(uint32_t sa, uint32_t a, uint32_t b) {
@@ -238,18 +245,20 @@ __device__ __forceinline__ void kp_sts128(uint32_t sa, uint32_t a, uint32_t b, u
 
 template <int FMT, int HD, bool SPLIT>
 __global__ void __launch_bounds__(KP_THREADS, 1)
-    kv8_prefill_kernel(const KAttnArgs a) {
+    kv8_prefill_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
     using S = KPShape<HD, SPLIT>;
-    constexpr int ROWS = S::ROWS;
+    constexpr int ROWS = S::ROWS, LINE = HD == 64 ? 64 : 128;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     const uint32_t sbase = smem_u32(smem);
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + S::O_BAR);
     uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = bar + 4, *v_full = bar + 6, *v_empty = bar + 8, *s_full = bar + 10,
-             *p_full = bar + 12, *o_full = bar + 14, *seg_done = bar + 15, *prep_full = bar + 16, *prep_empty = prep_full + KP_SLOTS;
+             *p_full = bar + 12, *o_full = bar + 14, *seg_done = bar + 15, *prep_full = bar + 16, *prep_empty = prep_full + KP_SLOTS,
+             *raw_full = bar + 24, *raw_empty = bar + 26;
     int* s_misc = reinterpret_cast<int*>(smem + S::O_MISC);
     float* s_prep = reinterpret_cast<float*>(smem + S::O_PREP);
+    int* s_row = reinterpret_cast<int*>(smem + S::O_PREP + KP_SLOTS * 96);
 
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
@@ -260,12 +269,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             mbar_init(&v_empty[s], 1);
             mbar_init(&s_full[s], 1);
             mbar_init(&p_full[s], 4);
+            mbar_init(&raw_full[s], 1);
+            mbar_init(&raw_empty[s], 4);
         }
         mbar_init(o_full, 1);
         mbar_init(seg_done, 8);
         for (int s = 0; s < KP_SLOTS; ++s) {
             mbar_init(&prep_full[s], 1);
-            mbar_init(&prep_empty[s], 12);
+            mbar_init(&prep_empty[s], 9);
         }
         fence_barrier_init();
     }
@@ -348,11 +359,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
 
     if (warp >= KP_W_CONV && warp < KP_W_PREP) {
         // ---------------------------------------------------------------- codes -> fp16 operands
-        // 8 keys x 64 channels a warp and step; rows r and r ^ 5 side by side: the stores of a quarter-warp do not meet on a bank.
-        // Items are K, V, K, V, ... of the tiles. A thread copies its own 16-byte pieces two items ahead and reads them back.
-        constexpr int HALF = HD / 64, STEPS = KP_KT / 8 * HALF / 4;
-        const int cw = warp - KP_W_CONV, r8 = (lane >> 3) ^ ((lane >> 2 & 1) * 5), P = a.c.page_tokens;
-        const uint32_t stage = sbase + S::O_RAW + (cw * 32 + lane) * 16;
+        // 8 keys x 64 channels a warp and step; rows r and r ^ 5 side by side: neither the loads nor the stores of a
+        // quarter-warp meet on a bank (the staged codes are swizzled too)
+        constexpr int HALF = HD / 64, STEPS = KP_KT / 8 * HALF / 4, STEP_ROWS = 4 / HALF * 8;
+        const int cw = warp - KP_W_CONV, r8 = (lane >> 3) ^ ((lane >> 2 & 1) * 5);
+        // this thread's row in the first step, its place in the operand and in the stage
+        const int row0 = (cw / HALF) * 8 + r8, half = cw % HALF, c16 = half * 4 + (lane & 3);
+        const uint32_t dst0 = (uint32_t)(half * (KP_KT * 128) + row0 * 128 + (((2 * (lane & 3)) ^ r8) << 4));
+        const uint32_t raw0 = sbase + S::O_RAW + (HD == 64 ? (uint32_t)(row0 * 64 + ((c16 ^ ((row0 >> 1) & 3)) << 4))
+                                                           : (uint32_t)(row0 * 128 + ((c16 ^ r8) << 4)));
         uint32_t it = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
@@ -360,54 +375,74 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             // the tiles that some row sees follow one another
             const int t0 = max(g.tile0, min(g.hi[0] < 0 ? INT_MAX : g.lo[0], g.hi[1] < 0 ? INT_MAX : g.lo[1]));
             const int t1 = min(g.tile0 + g.cnt - 1, max(g.hi[0], g.hi[1]));
-            const int n_items = 2 * max(0, t1 - t0 + 1);
-            for (int n = -2; n < n_items; ++n) {
-                const uint32_t t = it + (uint32_t)(n >> 1), b = t & 1u;  // the tile's count
-                const int v = n & 1;
-                if (n >= 0) {
-                    cp_async_wait_group<1>();
-                    if (t >= 2) wait((v ? v_empty : k_empty) + b, (t >> 1) - 1);
+            for (int kt = t0; kt <= t1; ++kt, ++it) {
+                const uint32_t b = it & 1u;
+                const int lo = any_lo - kt * KP_KT - row0, hi = g.q.kv - kt * KP_KT - row0;
+                const bool edge = hi + row0 < KP_KT || lo + row0 > 0;  // keys there may hold anything: they count as zero
+#pragma unroll 1
+                for (int v = 0; v < 2; ++v) {
+                    wait(&raw_full[v], it);
+                    if (it >= 2) wait((v ? v_empty : k_empty) + b, (it >> 1) - 1);
                     __syncwarp();
-                    const uint32_t op = sbase + (v ? S::O_V : S::O_K) + b * S::OP, raw = stage + v * S::RAW;
-#pragma unroll 2
-                    for (int i = 0; i < STEPS; ++i) {
-                        const int row = ((i * 4 + cw) / HALF) * 8 + r8, half = (i * 4 + cw) % HALF;
-                        const uint4 x = lds128(raw + i * 2048);
-                        const uint32_t y[4] = {kd_bias<FMT>(x.x), kd_bias<FMT>(x.y), kd_bias<FMT>(x.z), kd_bias<FMT>(x.w)};
-                        const uint32_t dst = op + (uint32_t)(half * (KP_KT * 128) + row * 128);
+                    const uint32_t op = sbase + (v ? S::O_V : S::O_K) + b * S::OP + dst0, raw = raw0 + v * S::RAW;
+#pragma unroll 1
+                    for (int i0 = 0; i0 < STEPS; i0 += 4) {
+                        uint4 x[4];
 #pragma unroll
-                        for (int k = 0; k < 2; ++k)
-                            kp_sts128(dst + (((2 * (lane & 3) + k) ^ r8) << 4), kd_half2<FMT>(y[2 * k], false),
-                                      kd_half2<FMT>(y[2 * k], true), kd_half2<FMT>(y[2 * k + 1], false), kd_half2<FMT>(y[2 * k + 1], true));
+                        for (int i = 0; i < 4; ++i) x[i] = lds128(raw + (i0 + i) * (STEP_ROWS * LINE));
+                        if (edge) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                if ((i0 + i) * STEP_ROWS >= hi || (i0 + i) * STEP_ROWS < lo) x[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        const uint32_t dst = op + i0 * (STEP_ROWS * 128);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t y[4] = {kd_bias<FMT>(x[i].x), kd_bias<FMT>(x[i].y), kd_bias<FMT>(x[i].z), kd_bias<FMT>(x[i].w)};
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                kp_sts128((dst + i * (STEP_ROWS * 128)) ^ (k << 4), kd_half2<FMT>(y[2 * k], false),
+                                          kd_half2<FMT>(y[2 * k], true), kd_half2<FMT>(y[2 * k + 1], false),
+                                          kd_half2<FMT>(y[2 * k + 1], true));
+                        }
                     }
                     kp_fence_async();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive((v ? v_full : k_full) + b);
-                }
-                if (n + 2 < n_items) {
-                    const uint32_t slot = (t + 1) % KP_SLOTS;
-                    const int key0 = (t0 + ((n + 2) >> 1)) * KP_KT;
-                    if (!v) wait(&prep_full[slot], (t + 1) / KP_SLOTS);
-                    const int* first = reinterpret_cast<const int*>(s_prep + slot * 32 + 24);
-                    const uint8_t* codes = static_cast<const uint8_t*>(v ? a.c.v : a.c.k);
-#pragma unroll 2
-                    for (int i = 0; i < STEPS; ++i) {
-                        const int row = ((i * 4 + cw) / HALF) * 8 + r8, half = (i * 4 + cw) % HALF, key = key0 + row;
-                        const bool in = key < g.q.kv && key >= any_lo;  // keys that no row sees may hold anything: they count as zero
-                        const uint8_t* src = codes + ((long long)first[row >> 4] * P + (key & (P - 1))) * HD + half * 64 + (lane & 3) * 16;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(stage + v * S::RAW + i * 2048), "l"(src),
-                                     "r"(in ? 16 : 0)
-                                     : "memory");
+                    if (lane == 0) {
+                        mbar_arrive(&raw_empty[v]);
+                        mbar_arrive((v ? v_full : k_full) + b);
                     }
-                    __syncwarp();
-                    if (v && lane == 0) mbar_arrive(&prep_empty[slot]);
                 }
-                cp_async_commit();
             }
-            it += (uint32_t)(n_items / 2);
             cur += g.cnt;
         }
-        cp_async_wait_all();
+    } else if (warp == KP_W_LOAD) {
+        // ---------------------------------------------------------------- codes into the stages
+        const int box = min(a.c.page_tokens, 64), boxes = KP_KT / box;
+        uint32_t it = 0;
+        for (int cur = begin; cur < end;) {
+            const KPSeg g = walk.seek(a, cur, end);
+            for (int j = 0; j < g.cnt; ++j) {
+                const int kt = g.tile0 + j;
+                if (!kp_active<SPLIT>(g, 0, kt) && !kp_active<SPLIT>(g, 1, kt)) continue;
+                const uint32_t slot = it % KP_SLOTS;
+                wait(&prep_full[slot], it / KP_SLOTS);
+                const bool load = lane < boxes && kt * KP_KT + lane * box < g.q.kv;
+                const int y = load ? s_row[slot * 8 + lane * (box / 16)] : 0, n = __popc(__ballot_sync(0xffffffffu, load));
+                if (lane == 0) mbar_arrive(&prep_empty[slot]);
+#pragma unroll 1
+                for (int v = 0; v < 2; ++v) {
+                    if (it > 0) wait(&raw_empty[v], it - 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive_expect_tx(&raw_full[v], (uint32_t)(n * box * HD));
+                    __syncwarp();
+                    if (load) kd_tma(sbase + S::O_RAW + v * S::RAW + lane * box * LINE, v ? &tm_v : &tm_k, 0, y, &raw_full[v]);
+                }
+                ++it;
+            }
+            cur += g.cnt;
+        }
     } else if (warp == KP_W_PREP) {
         // ---------------------------------------------------------------- pages and scales of 8 x 16 keys, some tiles ahead
         uint32_t it = 0;
@@ -440,11 +475,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     } else if (vs != 0.f) {
                         ks = __uint_as_float(0x7fffffffu);  // NaN for whoever sees these keys
                     }
-                    float* d = s_prep + slot * 32;
+                    float* d = s_prep + slot * 24;
                     d[lane] = ks;
                     d[8 + lane] = lv;
                     d[16 + lane] = rv;
-                    reinterpret_cast<int*>(d)[24 + lane] = unit;
+                    s_row[slot * 8 + lane] = unit * a.c.page_tokens + (key & (a.c.page_tokens - 1));
                 }
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&prep_full[slot]);
@@ -455,6 +490,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     } else if (warp == KP_W_MMA) {
         // ---------------------------------------------------------------- products
         constexpr uint32_t id_s = tg_idesc(128, KP_KT), id_o = tg_idesc(128, HD) | (1u << 16);  // V: MN-major
+        const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0}, segs = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
@@ -468,19 +504,22 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 wait(&p_full[s], np[s]++);
                 __syncwarp();
                 kp_fence_after();
-                if (lane == 0 && ok) {
-                    const uint32_t vop = sbase + S::O_V + b * S::OP;
-#pragma unroll 1
-                    for (int x = 0; x < (SPLIT ? 2 : 1); ++x) {
-#pragma unroll 1
-                        for (int k = 0; k < KP_KT / 16; ++k)
-                            kp_mma_ts(tmem + 256 + 128 * s, tmem + 128 * s + (k >> 1) * 32 + x * 16 + (k & 1) * 8,
-                                      kp_desc_mn(vop + k * 2048, KP_KT * 128), id_o, have_o[s] || x > 0 || k > 0);
-                    }
-                }
+                ok = __all_sync(0xffffffffu, ok);
+                const uint32_t bu = __shfl_sync(0xffffffffu, b, 0), add = __shfl_sync(0xffffffffu, (uint32_t)have_o[s], 0);
                 have_o[s] = true;
                 left -= 1u << (8 * b);
-                if (((left >> (8 * b)) & 255u) == 0 && lane == 0 && ok) kp_commit(&v_empty[b]);
+                const bool free = ((left >> (8 * b)) & 255u) == 0;
+                if (ok && kp_elect()) {
+                    const uint64_t db = kp_desc_mn(sbase + S::O_V + bu * S::OP, KP_KT * 128);
+#pragma unroll
+                    for (int x = 0; x < (SPLIT ? 2 : 1); ++x)
+#pragma unroll
+                        for (int k = 0; k < KP_KT / 16; ++k)  // 16 keys: 2048 bytes further
+                            kp_mma_ts(tm + 256 + 128 * s, tm + 128 * s + (k >> 1) * 32 + x * 16 + (k & 1) * 8, db + k * 128, id_o,
+                                      x > 0 || k > 0 ? 1u : add);
+                    if (free) kp_commit(&v_empty[bu]);
+                }
+                __syncwarp();
                 pend[s] = -1;
             };
             auto score = [&](auto stream, uint32_t b) {  // S_s = Q_s . K^T
@@ -493,18 +532,28 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 wait(&k_full[b], it >> 1);
                 __syncwarp();
                 kp_fence_after();
-                if (lane == 0 && ok) {
-                    const uint32_t kop = sbase + S::O_K + b * S::OP;
-#pragma unroll 1
-                    for (int x = SPLIT ? 1 : 0; x >= 0; --x) {  // the low parts first
-                        const uint32_t qop = sbase + S::O_Q + (SPLIT ? x : s) * S::Q_TILE;
-#pragma unroll 1
-                        for (int k = 0; k < HD / 16; ++k)
-                            kp_mma_ss(tmem + 128 * s, tg_desc(qop + (k >> 2) * 128 * 128 + (k & 3) * 32),
-                                      tg_desc(kop + (k >> 2) * KP_KT * 128 + (k & 3) * 32), id_s, (SPLIT && x == 0) || k > 0);
+                ok = __all_sync(0xffffffffu, ok);
+                const uint32_t bu = __shfl_sync(0xffffffffu, b, 0);
+                if (ok && kp_elect()) {
+                    const uint64_t db = tg_desc(sbase + S::O_K + bu * S::OP);
+                    // 16 channels: 32 bytes further, 64 channels: the next slab; the low parts of q first
+                    if (SPLIT) {
+                        const uint64_t da = tg_desc(sbase + S::O_Q + S::Q_TILE);
+                        kp_mma_ss<false>(tm + 128 * s, da, db, id_s);
+#pragma unroll
+                        for (int k = 1; k < HD / 16; ++k)
+                            kp_mma_ss<true>(tm + 128 * s, da + ((k >> 2) * 128 * 128 + (k & 3) * 32) / 16,
+                                            db + ((k >> 2) * KP_KT * 128 + (k & 3) * 32) / 16, id_s);
                     }
+                    const uint64_t da = tg_desc(sbase + S::O_Q + (SPLIT ? 0 : s) * S::Q_TILE);
+                    kp_mma_ss<SPLIT>(tm + 128 * s, da, db, id_s);
+#pragma unroll
+                    for (int k = 1; k < HD / 16; ++k)
+                        kp_mma_ss<true>(tm + 128 * s, da + ((k >> 2) * 128 * 128 + (k & 3) * 32) / 16,
+                                        db + ((k >> 2) * KP_KT * 128 + (k & 3) * 32) / 16, id_s);
                     kp_commit(&s_full[s]);
                 }
+                __syncwarp();
                 pend[s] = (int)it;
             };
             constexpr std::integral_constant<int, 0> st0{};
@@ -519,7 +568,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 if (pend[1] >= 0 && (!SPLIT || act1)) weigh(st1);
                 if (act1) score(st1, b);
                 left += ((act0 ? 1u : 0u) + (act1 ? 1u : 0u)) << (8 * b);
-                if (lane == 0 && ok) kp_commit(&k_empty[b]);
+                if (ok && kp_elect()) kp_commit(&k_empty[b]);
+                __syncwarp();
                 ++it;
             }
             // the last tiles' weights, in the order of the tiles
@@ -530,7 +580,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             if (segs > 0) wait(seg_done, segs - 1);
             ++segs;
             __syncwarp();
-            if (lane == 0 && ok) kp_commit(o_full);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok && kp_elect()) kp_commit(o_full);
             __syncwarp();
             cur += g.cnt;
         }
@@ -667,7 +718,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 wait(&s_full[s], n_s++);
                 __syncwarp();
                 kp_fence_after();
-                const float* pr = s_prep + slot * 32;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
+                const float* pr = s_prep + slot * 24;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
                 // Loops of 32 columns, not unrolled: the roles' code has to share the instruction cache.
                 const bool edge = key0 + KP_KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
                 uint32_t bad = 0;  // of an edge tile: blocks of 16 keys with a scale that is no number, of which this row sees some
