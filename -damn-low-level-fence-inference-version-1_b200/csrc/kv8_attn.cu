@@ -53,14 +53,29 @@ template <int FMT, int HD, bool SPLIT>
 static int kv8_launch_prefill(const KAttnArgs& p, cudaStream_t st) {
     using S = KPShape<HD, SPLIT>;
     static int done[64] = {};
-    CUtensorMap tm_k, tm_v;
+    CUtensorMap tm_q, tm_k, tm_v;
     const int box = p.c.page_tokens < 64 ? p.c.page_tokens : 64;
     if (!kv8_tensor_map(&tm_k, &p.c, p.c.k, box) || !kv8_tensor_map(&tm_v, &p.c, p.c.v, box))
         return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the cache");
+    const long long rows = (long long)p.n_tokens * p.n_q_heads;
+    if (!tg_tensor_map(&tm_q, p.q_rows, (int)(rows * (SPLIT ? 2 : 1)), HD, 128))
+        return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the query rows");
+    kv8_q_rows_kernel<HD, SPLIT><<<(unsigned)((rows + KQ_WARPS - 1) / KQ_WARPS), 32 * KQ_WARPS, 0, st>>>(p);
+    FENCE_CUDA_TRY(cudaGetLastError());
     auto kern = kv8_prefill_kernel<FMT, HD, SPLIT>;
     FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM, done));
-    kern<<<KP_SMS, KP_THREADS, S::SMEM, st>>>(p, tm_k, tm_v);
-    return cuda_status(cudaGetLastError(), "kv8_attention");
+    // its set-up runs beside the q rows' kernel; it waits for that one before it reads them
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(KP_SMS);
+    cfg.blockDim = dim3(KP_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, kern, p, tm_q, tm_k, tm_v), "kv8_attention");
 }
 
 constexpr size_t KV8_ARRIVED_BYTES = 4096;  // counters, at the workspace's start: 2048 for each kernel
@@ -70,19 +85,31 @@ constexpr int KV8_DECODE_ROWS = 16;         // the most query rows per KV head o
 static bool kv8_has_prefill(const fence_kv8_cache* c, const fence_kv8_attn* a) {
     return c->head_dim <= 128 && (long long)a->max_new * (a->n_q_heads / c->n_kv_heads) > KV8_DECODE_ROWS;
 }
+// The workspace: counters, the decode kernel's partial results, the prefill kernel's, its query rows and their scales.
+static size_t kv8_prefill_part_bytes(const fence_kv8_cache* c) {
+    return (size_t)KP_SMS * 4 * 128 * (c->head_dim + 2) * sizeof(float);
+}
+static size_t kv8_q_rows_bytes(const fence_kv8_cache* c, const fence_paged_batch* b, const fence_kv8_attn* a) {
+    return ((size_t)b->n_tokens * a->n_q_heads * c->head_dim * 2 * (a->type == FENCE_F32 ? 2 : 1) + 255) & ~(size_t)255;
+}
 static size_t kv8_decode_part_bytes(const fence_kv8_cache* c) {
     return (size_t)KV8_SMS * 2 * 2 * 16 * (c->head_dim + 2) * sizeof(float);
 }
 
 template <int FMT, int HD>
-static int kv8_launch_attn(const KAttnArgs& pd, bool split, int nt, bool prefill, char* ws, cudaStream_t st) {
+static int kv8_launch_attn(const KAttnArgs& pd, bool split, int nt, bool prefill, char* ws, size_t q_bytes,
+                           cudaStream_t st) {
     KAttnArgs p = pd;
     if constexpr (HD <= 128) {
         if (prefill) {
             // one request: the prefill kernel takes it whatever its length is
             p.min_rows = p.n_req == 1 ? 0 : KV8_DECODE_ROWS;
             p.arrived = reinterpret_cast<int*>(ws + 2048);
-            p.part = reinterpret_cast<float*>(ws + KV8_ARRIVED_BYTES + kv8_decode_part_bytes(&p.c));
+            char* at = ws + KV8_ARRIVED_BYTES + kv8_decode_part_bytes(&p.c);
+            p.part = reinterpret_cast<float*>(at);
+            at += kv8_prefill_part_bytes(&p.c);
+            p.q_rows = reinterpret_cast<__half*>(at);
+            p.q_scale = reinterpret_cast<float*>(at + q_bytes);
             const int e = split ? kv8_launch_prefill<FMT, HD, true>(p, st) : kv8_launch_prefill<FMT, HD, false>(p, st);
             if (e || p.n_req == 1) return e;
             p.max_rows = KV8_DECODE_ROWS;
@@ -102,6 +129,8 @@ static int kv8_attn_check(const fence_kv8_cache* c, const fence_paged_batch* b, 
         return set_error(FENCE_E_ARG, "%s: %d query heads over %d kv heads", who, a->n_q_heads, c->n_kv_heads);
     if (!kv8_type_ok(a->type)) return set_error(FENCE_E_UNSUPPORTED, "%s: element type %d", who, a->type);
     if (!(a->scale >= 0.f && a->scale < INFINITY)) return set_error(FENCE_E_ARG, "%s: scale %g", who, (double)a->scale);
+    if ((long long)b->n_tokens * a->n_q_heads > INT_MAX / 2)
+        return set_error(FENCE_E_UNSUPPORTED, "%s: more than 2^30 query rows", who);
     if (a->max_new <= 0) return set_error(FENCE_E_ARG, "%s: max_new %d", who, a->max_new);
     return FENCE_OK;
 }
@@ -113,7 +142,8 @@ extern "C" size_t fence_kv8_attention_workspace_bytes(const fence_kv8_cache* c, 
     using namespace fence;
     if (kv8_attn_check(c, b, a, "kv8_attention_workspace_bytes")) return 0;
     size_t n = KV8_ARRIVED_BYTES + kv8_decode_part_bytes(c);
-    if (kv8_has_prefill(c, a)) n += (size_t)KP_SMS * 4 * 128 * (c->head_dim + 2) * sizeof(float);
+    if (kv8_has_prefill(c, a))
+        n += kv8_prefill_part_bytes(c) + kv8_q_rows_bytes(c, b, a) + (size_t)b->n_tokens * a->n_q_heads * sizeof(float);
     return n;
 }
 
@@ -138,19 +168,21 @@ extern "C" int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_b
     KAttnArgs p{*c, b->block_table, b->kv_len, b->new_start, b->n_req, b->n_tokens, b->max_pages, ilog2(c->page_tokens),
                 a->n_q_heads / c->n_kv_heads, a->n_q_heads, a->window > 0 ? a->window : 0, a->type, a->q, a->out, a->lse,
                 a->q_stride, a->out_stride, (float)(a->scale * 1.4426950408889634), INT_MAX, 0, kv8_wide(a->q, a->q_stride, a->type),
-                kv8_wide(a->out, a->out_stride, a->type), static_cast<int*>(a->workspace),
+                kv8_wide(a->out, a->out_stride, a->type), nullptr, nullptr, static_cast<int*>(a->workspace),
                 reinterpret_cast<float*>(static_cast<char*>(a->workspace) + KV8_ARRIVED_BYTES)};
     const bool split = a->type == FENCE_F32, prefill = kv8_has_prefill(c, a);
     const int nt = (long long)a->max_new * p.G <= 8 ? 1 : 2;
     const cudaStream_t st = (cudaStream_t)stream;
+    char* ws = static_cast<char*>(a->workspace);
+    const size_t q_bytes = kv8_q_rows_bytes(c, b, a);
     const int kind = (c->format == KV8_E4M3 ? 3 : 0) + (c->head_dim == 64 ? 0 : c->head_dim == 128 ? 1 : 2);
     switch (kind) {
-        case 0: return kv8_launch_attn<KV8_INT8, 64>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
-        case 1: return kv8_launch_attn<KV8_INT8, 128>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
-        case 2: return kv8_launch_attn<KV8_INT8, 256>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
-        case 3: return kv8_launch_attn<KV8_E4M3, 64>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
-        case 4: return kv8_launch_attn<KV8_E4M3, 128>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
-        default: return kv8_launch_attn<KV8_E4M3, 256>(p, split, nt, prefill, static_cast<char*>(a->workspace), st);
+        case 0: return kv8_launch_attn<KV8_INT8, 64>(p, split, nt, prefill, ws, q_bytes, st);
+        case 1: return kv8_launch_attn<KV8_INT8, 128>(p, split, nt, prefill, ws, q_bytes, st);
+        case 2: return kv8_launch_attn<KV8_INT8, 256>(p, split, nt, prefill, ws, q_bytes, st);
+        case 3: return kv8_launch_attn<KV8_E4M3, 64>(p, split, nt, prefill, ws, q_bytes, st);
+        case 4: return kv8_launch_attn<KV8_E4M3, 128>(p, split, nt, prefill, ws, q_bytes, st);
+        default: return kv8_launch_attn<KV8_E4M3, 256>(p, split, nt, prefill, ws, q_bytes, st);
     }
 }
 

@@ -41,6 +41,8 @@ struct KAttnArgs {
     int max_rows;      // decode kernel: requests of more query rows per KV head are left to the prefill kernel
     int min_rows;      // prefill kernel: requests of at most this many are the decode kernel's
     int q_wide, out_wide;  // rows are 16-byte aligned
+    __half* q_rows;        // prefill kernel: [2][n_kv_heads][n_tokens * G][head_dim], rows of q as it multiplies them (high, low)
+    float* q_scale;        // [n_kv_heads][n_tokens * G]: times this gives scores
     int* arrived;      // [CTAs] partial results of the unit that starts in this CTA and goes on in the next
     float* part;       // [CTAs][2][rows * (head_dim + 2)]
 };

@@ -49,6 +49,73 @@ struct KPShape {
     static constexpr int REC = 128 * (HD + 2);  // floats of one stream's partial result
 };
 
+// The rows of q as the prefill kernel multiplies them, in its order (KV head, token, query head of the KV head): by a power of
+// two into [256, 512), so that fp16 holds them whatever their range is, and what fp16 leaves of them (SPLIT). A pass of
+// its own over q: done by the softmax warps at each unit's start it took them 9 us every time (short of independent
+// work, with code that the tiles' loops had pushed out of the instruction cache), and TMA can fetch the finished rows while
+// the unit before ends. A warp per row.
+constexpr int KQ_WARPS = 8;
+template <int HD, bool SPLIT>
+__global__ void __launch_bounds__(32 * KQ_WARPS) kv8_q_rows_kernel(const KAttnArgs a) {
+    pdl_launch_dependents();
+    constexpr int EPL = HD / 32;
+    const int lane = threadIdx.x & 31;
+    const long long i = (long long)blockIdx.x * KQ_WARPS + (threadIdx.x >> 5), per_head = (long long)a.n_tokens * a.G;
+    if (i >= per_head * a.c.n_kv_heads) return;
+    const int tok = (int)(i / a.n_q_heads), head = (int)(i % a.n_q_heads);  // in q's order
+    const long long src = tok * a.q_stride + (long long)head * HD + lane * EPL;
+    float x[EPL];
+    if (SPLIT) {
+        const float* p = static_cast<const float*>(a.q) + src;
+        if (a.q_wide && EPL == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            x[0] = v.x, x[1] = v.y, x[EPL - 2] = v.z, x[EPL - 1] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) x[e] = p[e];
+        }
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(a.q) + src;
+        uint32_t w[EPL / 2];
+        if (a.q_wide && EPL == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(p);
+            w[0] = v.x, w[EPL / 2 - 1] = v.y;
+        } else {
+#pragma unroll
+            for (int e = 0; e < EPL / 2; ++e) w[e] = (uint32_t)p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
+        }
+#pragma unroll
+        for (int e = 0; e < EPL / 2; ++e) {
+            if (a.type == FENCE_F16) {
+                x[2 * e] = half_bits_to_float(w[e]), x[2 * e + 1] = half_bits_to_float(w[e] >> 16);
+            } else {
+                x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+            }
+        }
+    }
+    uint32_t big = 0;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
+    big = __reduce_max_sync(0xffffffffu, big);
+    const int ex = (int)(big >> 23);
+    const bool plain = ex == 255;  // infinity or NaN in the row
+    const int sh = plain ? 0 : max(ex, 1) - 127 - 8;
+    const float f1 = __uint_as_float((uint32_t)(127 - max(min(sh, 126), -126)) << 23);
+    const float f2 = sh < -126 ? __uint_as_float((uint32_t)(1 - sh) << 23) : 1.f;
+    const int h = head / a.G;
+    const long long row = h * per_head + (long long)tok * a.G + (head - h * a.G);
+    if (lane == 0) a.q_scale[row] = (plain ? 1.f : ldexpf(1.f, sh)) * a.scale_log2;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(a.q_rows + row * HD) + lane * (EPL / 2);
+    uint32_t* low = dst + per_head * a.c.n_kv_heads * HD / 2;
+#pragma unroll
+    for (int e = 0; e < EPL; e += 2) {
+        const float u = x[e] * f1 * f2, v = x[e + 1] * f1 * f2;
+        const uint32_t hi = kd_pack(u, v);
+        dst[e / 2] = hi;
+        if (SPLIT) low[e / 2] = kd_pack_rest(u, v, hi);
+    }
+}
+
 // What every role derives for itself from the run's position.
 struct KPSeg {
     KReq q;
@@ -148,8 +215,12 @@ struct KPWalk {
 
 // Whether stream s has rows that see the tile of keys kt.
 template <bool SPLIT>
+__device__ __forceinline__ bool kp_active(int lo, int hi, int s, int kt) {
+    return kt >= lo && kt <= hi && (!SPLIT || (kt & 1) == s);
+}
+template <bool SPLIT>
 __device__ __forceinline__ bool kp_active(const KPSeg& g, int s, int kt) {
-    return kt >= g.lo[s] && kt <= g.hi[s] && (!SPLIT || (kt & 1) == s);
+    return kp_active<SPLIT>(g.lo[s], g.hi[s], s, kt);
 }
 
 #define KP_LD32(r, addr)                                                                                                     \
@@ -194,12 +265,11 @@ __device__ __forceinline__ void kp_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 // D (tensor memory) (+)= A (shared memory) . B^T, and the same with A in tensor memory
-template <bool ADD>
-__device__ __forceinline__ void kp_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc) {
+__device__ __forceinline__ void kp_mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, bool add) {
     asm volatile(
         "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(da), "l"(db), "r"(idesc), "n"(ADD ? 1 : 0)
+        "l"(da), "l"(db), "r"(idesc), "r"((uint32_t)add)
         : "memory");
 }
 __device__ __forceinline__ void kp_mma_ts(uint32_t d, uint32_t ta, uint64_t db, uint32_t idesc, uint32_t add) {
@@ -208,9 +278,6 @@ __device__ __forceinline__ void kp_mma_ts(uint32_t d, uint32_t ta, uint64_t db, 
         "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
         "r"(ta), "l"(db), "r"(idesc), "r"(add)
         : "memory");
-}
-__device__ __forceinline__ void kp_sts64(uint32_t sa, uint32_t a, uint32_t b) {
-    asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(sa), "r"(a), "r"(b) : "memory");
 }
 // two fp32 at once
 __device__ __forceinline__ uint64_t kp_two(float a, float b) {
@@ -245,7 +312,8 @@ __device__ __forceinline__ void kp_sts128(uint32_t sa, uint32_t a, uint32_t b, u
 
 template <int FMT, int HD, bool SPLIT>
 __global__ void __launch_bounds__(KP_THREADS, 1)
-    kv8_prefill_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
+    kv8_prefill_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v) {
     using S = KPShape<HD, SPLIT>;
     constexpr int ROWS = S::ROWS, LINE = HD == 64 ? 64 : 128;
     extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -255,14 +323,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + S::O_BAR);
     uint64_t *q_full = bar, *k_full = bar + 2, *k_empty = bar + 4, *v_full = bar + 6, *v_empty = bar + 8, *s_full = bar + 10,
              *p_full = bar + 12, *o_full = bar + 14, *seg_done = bar + 15, *prep_full = bar + 16, *prep_empty = prep_full + KP_SLOTS,
-             *raw_full = bar + 24, *raw_empty = bar + 26;
+             *raw_full = bar + 24, *raw_empty = bar + 26, *q_empty = bar + 28;
     int* s_misc = reinterpret_cast<int*>(smem + S::O_MISC);
     float* s_prep = reinterpret_cast<float*>(smem + S::O_PREP);
     int* s_row = reinterpret_cast<int*>(smem + S::O_PREP + KP_SLOTS * 96);
 
     if (tid == 0) {
         for (int s = 0; s < 2; ++s) {
-            mbar_init(&q_full[s], 4);
+            mbar_init(&q_full[s], 1);
             mbar_init(&k_full[s], 4);
             mbar_init(&k_empty[s], 1);
             mbar_init(&v_full[s], 4);
@@ -273,6 +341,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             mbar_init(&raw_empty[s], 4);
         }
         mbar_init(o_full, 1);
+        mbar_init(q_empty, 1);
         mbar_init(seg_done, 8);
         for (int s = 0; s < KP_SLOTS; ++s) {
             mbar_init(&prep_full[s], 1);
@@ -419,9 +488,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     } else if (warp == KP_W_LOAD) {
         // ---------------------------------------------------------------- codes into the stages
         const int box = min(a.c.page_tokens, 64), boxes = KP_KT / box;
-        uint32_t it = 0;
+        uint32_t it = 0, segs = 0;
+        pdl_wait();  // q's rows come from the kernel before
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
+            bool q_due = true;
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j;
                 if (!kp_active<SPLIT>(g, 0, kt) && !kp_active<SPLIT>(g, 1, kt)) continue;
@@ -440,7 +511,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     if (load) kd_tma(sbase + S::O_RAW + v * S::RAW + lane * box * LINE, v ? &tm_v : &tm_k, 0, y, &raw_full[v]);
                 }
                 ++it;
+                if (q_due && ok) {  // the unit's q rows, behind its first tile; once the last unit's scores are done
+                    q_due = false;
+                    if (segs > 0) wait(q_empty, segs - 1);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (ok && lane == 0) {
+                        const int per_head = a.n_tokens * a.G, y = g.h * per_head + g.q.start * a.G + g.row0;
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) {
+                            if (!SPLIT && max(g.lo[s], g.tile0) > min(g.hi[s], g.tile0 + g.cnt - 1)) continue;  // no rows here
+                            uint64_t* full = &q_full[SPLIT ? 0 : s];
+                            if (!SPLIT || s == 0) mbar_arrive_expect_tx(full, (SPLIT ? 2 : 1) * S::Q_TILE);
+#pragma unroll
+                            for (int x = 0; x < HD / 64; ++x)
+                                kd_tma(sbase + S::O_Q + s * S::Q_TILE + x * 128 * 128, &tm_q, x * 64,
+                                       SPLIT ? y + s * per_head * a.c.n_kv_heads : y + 128 * s, full);
+                        }
+                    }
+                    __syncwarp();
+                }
             }
+            ++segs;
             cur += g.cnt;
         }
     } else if (warp == KP_W_PREP) {
@@ -489,99 +580,84 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         }
     } else if (warp == KP_W_MMA) {
         // ---------------------------------------------------------------- products
+        // one copy of the code for both streams: it runs four times a tile and should find itself in the instruction cache
         constexpr uint32_t id_s = tg_idesc(128, KP_KT), id_o = tg_idesc(128, HD) | (1u << 16);  // V: MN-major
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-        uint32_t it = 0, nq[2] = {0, 0}, np[2] = {0, 0}, segs = 0;
+        uint32_t it = 0, nq = 0, np = 0, segs = 0;  // nq, np: 16 bits per stream, of which the lowest counts
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
-            int pend[2] = {-1, -1};          // the tile (count) whose weights stream s is making
-            bool have_q[2] = {false, false}, have_o[2] = {false, false};
-            uint32_t left = 0;               // streams that still need the V operand: 8 bits per buffer
-            auto weigh = [&](auto stream) {  // O_s += P_s . V of its pending tile
-                constexpr int s = decltype(stream)::value;
-                const uint32_t t = (uint32_t)pend[s], b = t & 1u;
-                wait(&v_full[b], t >> 1);
-                wait(&p_full[s], np[s]++);
-                __syncwarp();
-                kp_fence_after();
-                ok = __all_sync(0xffffffffu, ok);
-                const uint32_t bu = __shfl_sync(0xffffffffu, b, 0), add = __shfl_sync(0xffffffffu, (uint32_t)have_o[s], 0);
-                have_o[s] = true;
-                left -= 1u << (8 * b);
-                const bool free = ((left >> (8 * b)) & 255u) == 0;
-                if (ok && kp_elect()) {
-                    const uint64_t db = kp_desc_mn(sbase + S::O_V + bu * S::OP, KP_KT * 128);
-#pragma unroll
-                    for (int x = 0; x < (SPLIT ? 2 : 1); ++x)
-#pragma unroll
-                        for (int k = 0; k < KP_KT / 16; ++k)  // 16 keys: 2048 bytes further
-                            kp_mma_ts(tm + 256 + 128 * s, tm + 128 * s + (k >> 1) * 32 + x * 16 + (k & 1) * 8, db + k * 128, id_o,
-                                      x > 0 || k > 0 ? 1u : add);
-                    if (free) kp_commit(&v_empty[bu]);
-                }
-                __syncwarp();
-                pend[s] = -1;
-            };
-            auto score = [&](auto stream, uint32_t b) {  // S_s = Q_s . K^T
-                constexpr int s = decltype(stream)::value;
-                constexpr int qi = SPLIT ? 0 : s;
-                if (!have_q[qi]) {
-                    have_q[qi] = true;
-                    wait(&q_full[qi], nq[qi]++);
-                }
-                wait(&k_full[b], it >> 1);
-                __syncwarp();
-                kp_fence_after();
-                ok = __all_sync(0xffffffffu, ok);
-                const uint32_t bu = __shfl_sync(0xffffffffu, b, 0);
-                if (ok && kp_elect()) {
-                    const uint64_t db = tg_desc(sbase + S::O_K + bu * S::OP);
-                    // 16 channels: 32 bytes further, 64 channels: the next slab; the low parts of q first
-                    if (SPLIT) {
-                        const uint64_t da = tg_desc(sbase + S::O_Q + S::Q_TILE);
-                        kp_mma_ss<false>(tm + 128 * s, da, db, id_s);
-#pragma unroll
-                        for (int k = 1; k < HD / 16; ++k)
-                            kp_mma_ss<true>(tm + 128 * s, da + ((k >> 2) * 128 * 128 + (k & 3) * 32) / 16,
-                                            db + ((k >> 2) * KP_KT * 128 + (k & 3) * 32) / 16, id_s);
-                    }
-                    const uint64_t da = tg_desc(sbase + S::O_Q + (SPLIT ? 0 : s) * S::Q_TILE);
-                    kp_mma_ss<SPLIT>(tm + 128 * s, da, db, id_s);
-#pragma unroll
-                    for (int k = 1; k < HD / 16; ++k)
-                        kp_mma_ss<true>(tm + 128 * s, da + ((k >> 2) * 128 * 128 + (k & 3) * 32) / 16,
-                                        db + ((k >> 2) * KP_KT * 128 + (k & 3) * 32) / 16, id_s);
-                    kp_commit(&s_full[s]);
-                }
-                __syncwarp();
-                pend[s] = (int)it;
-            };
-            constexpr std::integral_constant<int, 0> st0{};
-            constexpr std::integral_constant<int, 1> st1{};
-            for (int j = 0; j < g.cnt; ++j) {
-                const int kt = g.tile0 + j;
-                const bool act0 = kp_active<SPLIT>(g, 0, kt), act1 = kp_active<SPLIT>(g, 1, kt);
-                if (!act0 && !act1) continue;
+            int pend0 = -1, pend1 = -1;      // the tile (count) whose weights a stream is making
+            uint32_t have = 0, left = 0;     // have: q (bits 0, 1) and o (2, 3) of the streams; left: streams that still need V, 8 bits per buffer
+            const int last = g.tile0 + g.cnt;
+            // one more round than tiles, two where the streams take turns, to finish the last weights
+            for (int kt = g.tile0; kt < last + (SPLIT ? 2 : 1); ++kt) {
                 const uint32_t b = it & 1u;
-                if (pend[0] >= 0 && (!SPLIT || act0)) weigh(st0);
-                if (act0) score(st0, b);
-                if (pend[1] >= 0 && (!SPLIT || act1)) weigh(st1);
-                if (act1) score(st1, b);
-                left += ((act0 ? 1u : 0u) + (act1 ? 1u : 0u)) << (8 * b);
-                if (ok && kp_elect()) kp_commit(&k_empty[b]);
-                __syncwarp();
-                ++it;
+                bool used = false;
+#pragma unroll 1
+                for (int s = 0; s < 2; ++s) {
+                    const bool act = kt < last && kp_active<SPLIT>(s ? g.lo[1] : g.lo[0], s ? g.hi[1] : g.hi[0], s, kt);
+                    const int p = s ? pend1 : pend0;
+                    if (p >= 0 && (!SPLIT || (kt & 1) == s)) {  // O_s += P_s . V of the pending tile
+                        const uint32_t pb = (uint32_t)p & 1u;
+                        wait(&v_full[pb], (uint32_t)p >> 1);
+                        wait(&p_full[s], np >> (16 * s));
+                        np ^= 1u << (16 * s);
+                        left -= 1u << (8 * pb);
+                        const uint32_t add = (have >> (2 + s)) & 1u;
+                        have |= 4u << s;
+                        kp_fence_after();
+                        const uint32_t d = __shfl_sync(0xffffffffu, tm + 256 + 128 * s, 0), ta = __shfl_sync(0xffffffffu, tm + 128 * s, 0);
+                        const uint64_t db = kp_desc_mn(__shfl_sync(0xffffffffu, sbase + S::O_V + pb * S::OP, 0), KP_KT * 128);
+                        if (kp_elect() && ok) {
+#pragma unroll
+                            for (int x = 0; x < (SPLIT ? 2 : 1); ++x)
+#pragma unroll
+                                for (int k = 0; k < KP_KT / 16; ++k)  // 16 keys: 2048 bytes further
+                                    kp_mma_ts(d, ta + (k >> 1) * 32 + x * 16 + (k & 1) * 8, db + k * 128, id_o, x > 0 || k > 0 ? 1u : add);
+                            if (((left >> (8 * pb)) & 255u) == 0) kp_commit(&v_empty[pb]);
+                        }
+                        if (s) pend1 = -1;
+                        else pend0 = -1;
+                    }
+                    if (act) {  // S_s = Q_s . K^T
+                        const int qi = SPLIT ? 0 : s;
+                        if (!((have >> qi) & 1u)) {
+                            have |= 1u << qi;
+                            wait(&q_full[qi], nq >> (16 * qi));
+                            nq ^= 1u << (16 * qi);
+                        }
+                        wait(&k_full[b], it >> 1);
+                        kp_fence_after();
+                        const uint32_t d = __shfl_sync(0xffffffffu, tm + 128 * s, 0);
+                        const uint64_t db = tg_desc(__shfl_sync(0xffffffffu, sbase + S::O_K + b * S::OP, 0));
+                        const uint64_t da = tg_desc(__shfl_sync(0xffffffffu, sbase + S::O_Q + qi * S::Q_TILE, 0));
+                        if (kp_elect() && ok) {
+                            // 16 channels: 32 bytes further, 64 channels: the next slab; the low parts of q first
+#pragma unroll
+                            for (int x = SPLIT ? 1 : 0; x >= 0; --x)
+#pragma unroll
+                                for (int k = 0; k < HD / 16; ++k)
+                                    kp_mma_ss(d, da + (x * S::Q_TILE + (k >> 2) * 128 * 128 + (k & 3) * 32) / 16,
+                                              db + ((k >> 2) * KP_KT * 128 + (k & 3) * 32) / 16, id_s, (SPLIT && x == 0) || k > 0);
+                            kp_commit(&s_full[s]);
+                        }
+                        if (s) pend1 = (int)it;
+                        else pend0 = (int)it;
+                        left += 1u << (8 * b);
+                        used = true;
+                    }
+                }
+                if (used) {
+                    if (kp_elect() && ok) kp_commit(&k_empty[b]);
+                    ++it;
+                }
             }
-            // the last tiles' weights, in the order of the tiles
-            if (pend[0] >= 0 && (pend[1] < 0 || pend[0] <= pend[1])) weigh(st0);
-            if (pend[1] >= 0) weigh(st1);
-            if (pend[0] >= 0) weigh(st0);
+            if (kp_elect() && ok) kp_commit(q_empty);
+            __syncwarp();
             // a stream without tiles here may still be at the last unit's end: o_full must not run two ahead of it
             if (segs > 0) wait(seg_done, segs - 1);
             ++segs;
-            __syncwarp();
-            ok = __all_sync(0xffffffffu, ok);
-            if (ok && kp_elect()) kp_commit(o_full);
+            if (kp_elect() && ok) kp_commit(o_full);
             __syncwarp();
             cur += g.cnt;
         }
@@ -590,6 +666,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         const int s = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_s = t_lane + 128 * s, t_o = t_lane + 256 + 128 * s;
         uint32_t n_s = 0, n_o = 0, it = 0;
+        pdl_wait();
         // rows that belong to no request
         if (a.min_rows == 0) {
             const int used = max(0, min(a.new_start[a.n_req], a.n_tokens));
@@ -612,95 +689,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             // tiles that all of this stream's rows see whole need no mask
             const int r_lo = g.row0 + (SPLIT ? 0 : 128 * s), r_hi = min(r_lo + 128, g.row0 + g.nrows) - 1;
             const int lim_first = g.q.kv - g.q.n + r_lo / a.G, lim_last = g.q.kv - g.q.n + r_hi / a.G;
-            // whether this stream's q operand is used here (SPLIT: the other stream's tiles use it too)
-            const bool any_q = max(g.lo[s], g.tile0) <= min(g.hi[s], g.tile0 + g.cnt - 1);
-            float qs = 1.f;
-            if (any_q) {
-                // ---- q: rows by a power of two into [256, 512), fp16 (and what fp16 leaves); all lanes on one row at a time
-                constexpr int EPL = HD / 32, BATCH = 8;
-                const long long at = tok * a.q_stride + (long long)head * HD;
-#pragma unroll 1
-                for (int r0 = 0; r0 < 32; r0 += BATCH) {
-                    uint32_t w[BATCH][SPLIT ? EPL : EPL / 2];
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        const long long src = __shfl_sync(0xffffffffu, at, r0 + i) + lane * EPL;
-                        const bool in = __shfl_sync(0xffffffffu, (int)valid, r0 + i);
-#pragma unroll
-                        for (int e = 0; e < (SPLIT ? EPL : EPL / 2); ++e) w[i][e] = 0;
-                        if (in) {
-                            if (SPLIT) {
-                                const uint32_t* p = static_cast<const uint32_t*>(a.q) + src;
-                                if (a.q_wide && EPL == 4) {
-                                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-                                    w[i][0] = v.x, w[i][1] = v.y, w[i][EPL - 2] = v.z, w[i][EPL - 1] = v.w;
-                                } else {
-#pragma unroll
-                                    for (int e = 0; e < EPL; ++e) w[i][e] = __ldg(p + e);
-                                }
-                            } else {
-                                const uint16_t* p = static_cast<const uint16_t*>(a.q) + src;
-                                if (a.q_wide && EPL == 4) {
-                                    const uint2 v = __ldg(reinterpret_cast<const uint2*>(p));
-                                    w[i][0] = v.x, w[i][EPL / 2 - 1] = v.y;
-                                } else {
-#pragma unroll
-                                    for (int e = 0; e < EPL / 2; ++e)
-                                        w[i][e] = (uint32_t)__ldg(p + 2 * e) | ((uint32_t)__ldg(p + 2 * e + 1) << 16);
-                                }
-                            }
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < BATCH; ++i) {
-                        float x[EPL];
-#pragma unroll
-                        for (int e = 0; e < EPL; e += 2) {
-                            if (SPLIT) {
-                                x[e] = __uint_as_float(w[i][SPLIT ? e : 0]), x[e + 1] = __uint_as_float(w[i][SPLIT ? e + 1 : 0]);
-                            } else if (a.type == FENCE_F16) {
-                                x[e] = half_bits_to_float(w[i][e / 2]), x[e + 1] = half_bits_to_float(w[i][e / 2] >> 16);
-                            } else {
-                                x[e] = __uint_as_float(w[i][e / 2] << 16), x[e + 1] = __uint_as_float(w[i][e / 2] & 0xffff0000u);
-                            }
-                        }
-                        uint32_t big = 0;
-#pragma unroll
-                        for (int e = 0; e < EPL; ++e) big = max(big, __float_as_uint(x[e]) & 0x7fffffffu);
-                        big = __reduce_max_sync(0xffffffffu, big);
-                        const int ex = (int)(big >> 23);
-                        const bool plain = ex == 255;
-                        const int sh = plain ? 0 : max(ex, 1) - 127 - 8;
-                        const float f1 = __uint_as_float((uint32_t)(127 - max(min(sh, 126), -126)) << 23);
-                        const float f2 = sh < -126 ? __uint_as_float((uint32_t)(1 - sh) << 23) : 1.f;
-                        if (lane == r0 + i) qs = (plain ? 1.f : ldexpf(1.f, sh)) * a.scale_log2;
-                        if (!SPLIT || s == 0) {
-                            const int qrow = (warp & 3) * 32 + r0 + i, c = lane * EPL;
-                            const uint32_t dst = sbase + S::O_Q + (SPLIT ? 0 : s * S::Q_TILE) + (c >> 6) * (128 * 128) + qrow * 128 +
-                                                 ((((c >> 3) & 7) ^ (qrow & 7)) << 4) + (c & 7) * 2;
-                            uint32_t hi[EPL / 2], lo[EPL / 2];
-#pragma unroll
-                            for (int e = 0; e < EPL; e += 2) {
-                                const float u = x[e] * f1 * f2, v = x[e + 1] * f1 * f2;
-                                hi[e / 2] = kd_pack(u, v);
-                                lo[e / 2] = SPLIT ? kd_pack_rest(u, v, hi[e / 2]) : 0u;
-                            }
-                            if (EPL == 4) {
-                                kp_sts64(dst, hi[0], hi[EPL / 2 - 1]);
-                                if (SPLIT) kp_sts64(dst + S::Q_TILE, lo[0], lo[EPL / 2 - 1]);
-                            } else {
-                                asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst), "r"(hi[0]) : "memory");
-                                if (SPLIT) asm volatile("st.shared.b32 [%0], %1;" ::"r"(dst + S::Q_TILE), "r"(lo[0]) : "memory");
-                            }
-                        }
-                    }
-                }
-                if (!SPLIT || s == 0) {
-                    kp_fence_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&q_full[SPLIT ? 0 : s]);
-                }
-            }
+            const float qs = valid ? a.q_scale[(long long)g.h * a.n_tokens * a.G + tok * a.G + (g.row0 + i_row) % a.G] : 1.f;
             float m = -INFINITY, l = 0.f, lvref = -INFINITY, vref = 0.f;
             bool have_o = false;
             for (int j = 0; j < g.cnt; ++j) {
@@ -747,21 +736,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     if (edge) f = f < INFINITY ? fmaxf(f, 1e-30f) : 1e-30f;
                     return f;
                 };
+                constexpr int CH = 32, NB = CH / 16;
                 float mt = -INFINITY, lvmax = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32];
-                    KP_LD32(x, t_s + 32 * c);
-                    const float f0 = factor(2 * c), f1 = factor(2 * c + 1);
-                    lvmax = fmaxf(lvmax, fmaxf(pr[8 + 2 * c], pr[9 + 2 * c]));
-                    kp_wait_ld();
-                    float y0 = __uint_as_float(x[0]), y1 = __uint_as_float(x[16]);
+                for (int c = 0; c < KP_KT; c += CH) {
+                    uint32_t x[CH];
 #pragma unroll
-                    for (int e = 1; e < 16; ++e) {
-                        y0 = fmaxf(y0, __uint_as_float(x[e]));
-                        y1 = fmaxf(y1, __uint_as_float(x[16 + e]));
+                    for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
+                    float f[NB];
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) {
+                        f[k] = factor(c / 16 + k);
+                        lvmax = fmaxf(lvmax, pr[8 + c / 16 + k]);
                     }
-                    mt = fmaxf(mt, fmaxf(y0 * f0, y1 * f1));
+                    kp_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) {
+                        float y = __uint_as_float(x[16 * k]);
+#pragma unroll
+                        for (int e = 1; e < 16; ++e) y = fmaxf(y, __uint_as_float(x[16 * k + e]));
+                        mt = fmaxf(mt, y * f[k]);
+                    }
                 }
                 const bool move_v = lvmax > lvref + 4.f;
                 if (__any_sync(0xffffffffu, move_v || mt > m + KD_LAZY)) {
@@ -790,13 +785,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 const float mm = m == -INFINITY ? 0.f : m, lv0 = lvref == -INFINITY ? 0.f : lvref;
                 // ---- weights, in place of the scores
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                    uint32_t x[32], hi[16], lo[16];
-                    KP_LD32(x, t_s + 32 * c);
-                    float cf[2], add[2], fb[2], fl[2];
+                for (int c = 0; c < KP_KT; c += CH) {
+                    uint32_t x[CH];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int b = 2 * c + k;
+                    for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
+                    float cf[NB], add[NB], fb[NB], fl[NB];
+#pragma unroll
+                    for (int k = 0; k < NB; ++k) {
+                        const int b = c / 16 + k;
                         const float d = pr[8 + b] - lv0;
                         const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it
                         cf[k] = factor(b);
@@ -807,25 +803,30 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     }
                     kp_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const uint64_t cf2 = kp_two(cf[k], cf[k]), add2 = kp_two(add[k], add[k]);
-                        uint64_t sum2 = 0;
+                    for (int h = 0; h < CH / 32; ++h) {
+                        uint32_t hi[16], lo[16];
 #pragma unroll
-                        for (int e = 0; e < 16; e += 2) {
-                            const float2 y = kp_both(
-                                kp_fma2(kp_two(__uint_as_float(x[16 * k + e]), __uint_as_float(x[16 * k + e + 1])), cf2, add2));
-                            float p0 = kd_exp2(y.x), p1 = kd_exp2(y.y);
-                            sum2 = kp_add2(sum2, kp_two(p0, p1));
-                            if (SPLIT) p0 *= fb[k], p1 *= fb[k];
-                            const int at = k * 8 + (e >> 1);
-                            hi[at] = kd_pack(p0, p1);
-                            if (SPLIT) lo[at] = kd_pack_rest(p0, p1, hi[at]);
+                        for (int k = 0; k < 2; ++k) {
+                            const int kb = 2 * h + k;
+                            const uint64_t cf2 = kp_two(cf[kb], cf[kb]), add2 = kp_two(add[kb], add[kb]);
+                            uint64_t sum2 = 0;
+#pragma unroll
+                            for (int e = 0; e < 16; e += 2) {
+                                const float2 y = kp_both(kp_fma2(
+                                    kp_two(__uint_as_float(x[16 * kb + e]), __uint_as_float(x[16 * kb + e + 1])), cf2, add2));
+                                float p0 = kd_exp2(y.x), p1 = kd_exp2(y.y);
+                                sum2 = kp_add2(sum2, kp_two(p0, p1));
+                                if (SPLIT) p0 *= fb[kb], p1 *= fb[kb];
+                                const int at = k * 8 + (e >> 1);
+                                hi[at] = kd_pack(p0, p1);
+                                if (SPLIT) lo[at] = kd_pack_rest(p0, p1, hi[at]);
+                            }
+                            const float2 sum = kp_both(sum2);
+                            l += (sum.x + sum.y) * fl[kb];
                         }
-                        const float2 sum = kp_both(sum2);
-                        l += (sum.x + sum.y) * fl[k];
+                        KP_ST16(t_s + c + h * 32, hi);
+                        if (SPLIT) KP_ST16(t_s + c + h * 32 + 16, lo);
                     }
-                    KP_ST16(t_s + c * 32, hi);
-                    if (SPLIT) KP_ST16(t_s + c * 32 + 16, lo);
                 }
                 kp_wait_st();
                 kp_fence_before();
