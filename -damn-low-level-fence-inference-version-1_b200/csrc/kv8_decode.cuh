@@ -6,7 +6,7 @@
 // into matrix operands fast enough.
 //
 //  * Work is the list of 64-key tiles of every (request, KV head, group of 8 NT query rows), cut into
-//    equal runs, one per CTA, whatever the lengths are: a CTA's run may begin and end inside a unit. Such a
+//    runs of equal cost, one per CTA, whatever the lengths are: a CTA's run may begin and end inside a unit. Such a
 //    unit's partial results go to the workspace and the last of its CTAs to arrive joins them in the
 //    order of the keys, so the result does not depend on timing.
 //  * One producer warp per CTA copies each tile's pages (TMA, 16 or more rows at a time, swizzled so
@@ -49,6 +49,7 @@ struct KAttnArgs {
 
 constexpr int KD_TILE = 64, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
 constexpr int KD_MIN_TILES = 2;  // tiles per CTA below which more CTAs only add joins
+constexpr int KD_UNIT = 4;       // a unit's start and end cost about as much as four tiles: counted so when the runs are cut
 constexpr float KD_LAZY = 8.f;   // the running maximum may lag by 2^8: fp16 weights stay below 2^16
 
 template <int HD, int NT>
@@ -181,7 +182,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
         long long sum = 0;
         for (int r = r0; r < r1; ++r) {
             const KReq q = kd_request(a, r, ROWS, KD_TILE, blockIdx.x == 0);
-            const long long w = (long long)q.n * a.G > a.max_rows ? 0 : (long long)q.tiles * q.groups * a.c.n_kv_heads;
+            const long long w = (long long)q.n * a.G > a.max_rows ? 0 : (long long)(q.tiles + KD_UNIT) * q.groups * a.c.n_kv_heads;
             s_pre[r] = (int)min(w, (long long)INT_MAX);
             sum += w;
         }
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
         __syncthreads();
     }
     const int total = s_pre[a.n_req];
-    const int per = max(KD_MIN_TILES, (int)(((long long)total + gridDim.x - 1) / gridDim.x));
+    const int per = max(KD_MIN_TILES + KD_UNIT, (int)(((long long)total + gridDim.x - 1) / gridDim.x));
     const int begin = (int)min((long long)total, (long long)blockIdx.x * per), end = min(total, begin + min(per, total - begin));
     // the request of the run's first tile
     int r = 0;
@@ -229,8 +230,9 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
         for (int cur = begin; cur < end;) {
             while (s_pre[r + 1] <= cur) ++r;
             const KReq q = kd_request(a, r, ROWS, KD_TILE, false);
-            const int unit = (cur - s_pre[r]) / q.tiles, first = (cur - s_pre[r]) - unit * q.tiles;
-            const int cnt = min(q.tiles - first, end - cur), h = unit / q.groups;
+            const int span = q.tiles + KD_UNIT, unit = (cur - s_pre[r]) / span, unit0 = s_pre[r] + unit * span;
+            const int first = max(0, cur - unit0 - KD_UNIT), cnt = min(q.tiles, end - unit0 - KD_UNIT) - first, h = unit / q.groups;
+            if (cnt <= 0) break;  // the run ends in this unit's start: its tiles are the next CTA's
             const int lo = a.window > 0 ? max(0, q.kv - q.n - a.window + 1) : 0;
             const int* table = a.block_table + (size_t)r * a.max_pages;
             int ids = 0, ids_at = -1;  // this lane's page id of a run of 32 pages
@@ -272,7 +274,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                 asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&full[s])) : "memory");
             }
             if (!ok) break;
-            cur += cnt;
+            cur = unit0 + KD_UNIT + first + cnt;
         }
         cp_async_wait_all();
         return;
@@ -292,8 +294,10 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
     for (int cur = begin; cur < end;) {
         while (s_pre[r + 1] <= cur) ++r;
         const KReq q = kd_request(a, r, ROWS, KD_TILE, false);
-        const int unit = (cur - s_pre[r]) / q.tiles, first = (cur - s_pre[r]) - unit * q.tiles;
-        const int cnt = min(q.tiles - first, end - cur), h = unit / q.groups, row0 = (unit - h * q.groups) * ROWS;
+        const int span = q.tiles + KD_UNIT, unit = (cur - s_pre[r]) / span, unit0 = s_pre[r] + unit * span;
+        const int first = max(0, cur - unit0 - KD_UNIT), cnt = min(q.tiles, end - unit0 - KD_UNIT) - first;
+        if (cnt <= 0) break;
+        const int h = unit / q.groups, row0 = (unit - h * q.groups) * ROWS;
         const int rows = min(ROWS, q.n * a.G - row0);  // row = token * G + head in the group
         // ---- q rows: scaled by a power of two into [256, 512), as B fragments
         for (int i = warp; i < ROWS; i += KD_WARPS) {
@@ -347,7 +351,6 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
         // keys that every row sees, and keys that some row sees
         const int lim_first = q.kv - q.n + row0 / a.G, lim_last = q.kv - q.n + (row0 + rows - 1) / a.G;
         const int all_lo = a.window > 0 ? lim_last - a.window + 1 : 0, any_lo = a.window > 0 ? lim_first - a.window + 1 : 0;
-        const bool full_rows = rows == ROWS;
         float o[MT][NT][4];
 #pragma unroll
         for (int i = 0; i < MT; ++i)
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                     }
                 }
                 // ---- scale, mask, the largest of each row
-                const bool masked = !full_rows || key0 + 15 > lim_first || (a.window > 0 && key0 < all_lo);
+                const bool masked = key0 + 15 > lim_first || (a.window > 0 && key0 < all_lo);
                 float p[NT][4];
                 const bool grow = sv > vref && sv < INFINITY;
                 bool move = grow;
@@ -570,8 +573,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
             return HD == 64 ? gg * 8 + 2 * i2 + e : (i2 >> 3) * 128 + gg * 16 + 2 * (i2 & 7) + e;
         };
         const bool whole = cnt == q.tiles;
-        const int unit0 = cur - first;  // the unit's first tile in the list
-        const int c_first = unit0 / per, c_last = (unit0 + q.tiles - 1) / per;
+        const int c_first = (unit0 + KD_UNIT) / per, c_last = (unit0 + KD_UNIT + q.tiles - 1) / per;
         const int stride = ROWS * (HD + 2);
         bool write = whole;
         if (!whole) {
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
             }
         }
         named_bar_sync(1, 32 * KD_WARPS);
-        cur += cnt;
+        cur = unit0 + KD_UNIT + first + cnt;
     }
 }
 
