@@ -37,7 +37,7 @@ constexpr int KV8_SMS = 148;
 
 template <int FMT, int HD, bool SPLIT, int NT>
 static int kv8_launch_decode(const KAttnArgs& p, cudaStream_t st) {
-    using S = KDShape<HD, NT>;
+    using S = KDShape<HD, SPLIT, NT>;
     static int done[64] = {};
     CUtensorMap tm_k, tm_v;
     const int box = p.c.page_tokens < KD_TILE ? p.c.page_tokens : KD_TILE;
@@ -45,7 +45,8 @@ static int kv8_launch_decode(const KAttnArgs& p, cudaStream_t st) {
         return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the cache");
     auto kern = kv8_decode_kernel<FMT, HD, SPLIT, NT>;
     FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM + 4 * (FENCE_PAGED_MAX_REQ + 1), done));
-    kern<<<KV8_SMS * S::CTAS, KD_THREADS, S::SMEM + 4 * (p.n_req + 1), st>>>(p, tm_k, tm_v);
+    const int smem = S::SMEM + 4 * (p.n_req + 1), fit = 228 * 1024 / (smem + 1024);  // many requests' prefix sums can cost a CTA
+    kern<<<KV8_SMS * (fit < S::CTAS ? fit : S::CTAS), KD_THREADS, smem, st>>>(p, tm_k, tm_v);
     return cuda_status(cudaGetLastError(), "kv8_attention");
 }
 
@@ -93,7 +94,7 @@ static size_t kv8_q_rows_bytes(const fence_kv8_cache* c, const fence_paged_batch
     return ((size_t)b->n_tokens * a->n_q_heads * c->head_dim * 2 * (a->type == FENCE_F32 ? 2 : 1) + 255) & ~(size_t)255;
 }
 static size_t kv8_decode_part_bytes(const fence_kv8_cache* c) {
-    return (size_t)KV8_SMS * 2 * 2 * 16 * (c->head_dim + 2) * sizeof(float);
+    return (size_t)KV8_SMS * 3 * 2 * 16 * (c->head_dim + 2) * sizeof(float);
 }
 
 template <int FMT, int HD>

@@ -52,10 +52,11 @@ constexpr int KD_MIN_TILES = 2;  // tiles per CTA below which more CTAs only add
 constexpr int KD_UNIT = 4;       // a unit's start and end cost about as much as four tiles: counted so when the runs are cut
 constexpr float KD_LAZY = 8.f;   // the running maximum may lag by 2^8: fp16 weights stay below 2^16
 
-template <int HD, int NT>
+template <int HD, bool SPLIT, int NT>
 struct KDShape {
-    static constexpr int CTAS = HD == 256 && NT == 2 ? 1 : 2;  // per SM; one where the sums take 128 registers
-    static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? 6 : NT == 2 ? 5 : 3;
+    // CTAs per SM, by the registers that the sums take
+    static constexpr int CTAS = HD == 256 ? (NT == 2 ? 1 : 2) : (HD == 128 && NT == 2 ? 2 : 3);
+    static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? (CTAS == 3 ? 4 : 6) : NT == 2 ? 5 : 3;
     static constexpr int KV_BYTES = KD_TILE * HD;
     static constexpr int STAGE = 2 * KV_BYTES;
     static constexpr int ROWS = 8 * NT;
@@ -64,7 +65,7 @@ struct KDShape {
     static constexpr int O_SCALE = STAGES * STAGE;
     static constexpr int O_BAR = O_SCALE + STAGES * 32;
     static constexpr int O_Q = O_BAR + 2 * STAGES * 8;
-    static constexpr int O_QS = O_Q + NT * 2 * (HD / 16) * 256;
+    static constexpr int O_QS = O_Q + NT * (SPLIT ? 2 : 1) * (HD / 16) * 256;
     static constexpr int O_ML = O_QS + ROWS * 4;
     static constexpr int O_SLAB = O_ML + KD_WARPS * ROWS * 8;
     static constexpr int O_SCAN = O_SLAB + ROWS * SLAB * 4;
@@ -150,9 +151,9 @@ __device__ __forceinline__ KReq kd_request(const KAttnArgs& a, int r, int rows_p
 }
 
 template <int FMT, int HD, bool SPLIT, int NT>
-__global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
+__global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
     kv8_decode_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v) {
-    using S = KDShape<HD, NT>;
+    using S = KDShape<HD, SPLIT, NT>;
     constexpr int ROWS = S::ROWS, KS = HD / 16, MT = HD / 16, HALVES = HD == 256 ? 2 : 1, LINE = HD == 64 ? 64 : 128;
     extern __shared__ __align__(128) uint8_t smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
     float* s_scale = reinterpret_cast<float*>(smem + S::O_SCALE);  // [stage][K 4, V 4]
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + S::O_BAR);
     uint64_t* empty = full + S::STAGES;
-    uint2* s_q = reinterpret_cast<uint2*>(smem + S::O_Q);  // [NT][high, low][KS][32]
+    uint2* s_q = reinterpret_cast<uint2*>(smem + S::O_Q);  // [NT][high, SPLIT: low][KS][32]
     float* s_qs = reinterpret_cast<float*>(smem + S::O_QS);
     float2* s_ml = reinterpret_cast<float2*>(smem + S::O_ML);  // [warp][ROWS]
     float* s_slab = reinterpret_cast<float*>(smem + S::O_SLAB);
@@ -329,7 +330,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                 const int half = c / 128, cc = c % 128;
                 const int ct = HD == 64 ? cc / 16 : cc / 32, j = HD == 64 ? (cc % 16) / 4 : half * 8 + (cc % 32) / 4;
                 uint32_t* dst = reinterpret_cast<uint32_t*>(s_q) +
-                                ((((i >> 3) * 2) * KS + j) * 32 + (i & 7) * 4 + ct) * 2 + ((c >> 1) & 1);
+                                ((((i >> 3) * (SPLIT ? 2 : 1)) * KS + j) * 32 + (i & 7) * 4 + ct) * 2 + ((c >> 1) & 1);
                 dst[0] = hi;
                 if (SPLIT) dst[KS * 64] = kd_pack_rest(u, v, hi);
             }
@@ -387,7 +388,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, NT>::CTAS)
                         const uint32_t a2 = kd_half2<FMT>(xa, true), a3 = kd_half2<FMT>(xb, true);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint2 b = s_q[((nt * 2) * KS + j) * 32 + lane];
+                            const uint2 b = s_q[((nt * (SPLIT ? 2 : 1)) * KS + j) * 32 + lane];
                             kd_mma(acc[nt][SPLIT ? 0 : w & 1], a0, a1, a2, a3, b.x, b.y);
                             if (SPLIT) {
                                 const uint2 bl = s_q[((nt * 2 + 1) * KS + j) * 32 + lane];
