@@ -11,10 +11,11 @@
 //    order of the keys, so the result does not depend on timing.
 //  * One producer warp per CTA copies each tile's pages (TMA, 16 or more rows at a time, swizzled so
 //    that all operand loads are free of bank conflicts) and their scales into a ring of stages.
-//  * Four consumer warps take 16 keys of a tile each, with a softmax state of their own: keys are the
+//  * Four consumer warps take the tiles in turn, each with a softmax state of its own: keys are the
 //    rows of the matrix products (S^T = K Q^T: 16 keys x 8 rows, O^T = V^T P^T: 16 channels x 8 rows),
 //    so 8 query rows fill the instruction and nothing is padded for grouped heads. A page holds 16 or
-//    more keys: a warp's scales are two numbers.
+//    more keys: 16 keys share their scales. (A tile shared by the warps, 16 keys each, spent a third
+//    more instructions on the softmax state per key.)
 //  * Codes become fp16 exactly. Scales never touch them: k_scale multiplies the scores, v_scale / (the
 //    largest v_scale so far) the weights. q rows are brought to [256, 512) by a power of two, so that
 //    fp16 holds them whatever their range. SPLIT (fp32 activations): q and the weights as a pair of
@@ -172,7 +173,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
     if (tid == 0) {
         for (int s = 0; s < S::STAGES; ++s) {
             mbar_init(&full[s], 33);
-            mbar_init(&empty[s], KD_WARPS);
+            mbar_init(&empty[s], 1);
         }
         fence_barrier_init();
     }
@@ -359,65 +360,100 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
             for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
         float vref = 0.f, vinv = 0.f;
 
-        for (int i = 0; i < cnt; ++i, ++it) {
-            const int s = it % S::STAGES, key0 = (q.tile0 + first + i) * KD_TILE + warp * 16;
-            if (ok) ok = mbar_wait(&full[s], (uint32_t)(it / S::STAGES) & 1u);
+        for (int i = warp; i < cnt; i += KD_WARPS) {
+            const uint32_t n = (uint32_t)(it + i);
+            const int s = n % S::STAGES, key0 = (q.tile0 + first + i) * KD_TILE;
+            if (ok) ok = mbar_wait(&full[s], (n / S::STAGES) & 1u);
             __syncwarp();
-            if (key0 <= lim_last && key0 + 15 >= any_lo && lim_last >= 0) {
+            if (key0 <= lim_last && key0 + KD_TILE - 1 >= any_lo && lim_last >= 0) {
+                constexpr int MK = KD_TILE / 16;  // blocks of 16 keys: one page each, or a part of one
                 const uint32_t kb = sbase + (uint32_t)(s * S::STAGE), vb = kb + S::KV_BYTES;
-                const int pi = (warp * 16) / box;
-                const float sk = s_scale[s * 8 + pi], sv = s_scale[s * 8 + 4 + pi];
-                // ---- scores of 16 keys
-                float acc[NT][2][4];
+                float sk[MK], sv[MK];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt)
+                for (int y = 0; y < MK; ++y) {
+                    sk[y] = s_scale[s * 8 + y * 16 / box];
+                    sv[y] = s_scale[s * 8 + 4 + y * 16 / box];
+                }
+                // ---- scores of 64 keys: four products side by side
+                float acc[MK][NT][4], low[SPLIT ? MK : 1][NT][4];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) acc[nt][c][0] = acc[nt][c][1] = acc[nt][c][2] = acc[nt][c][3] = 0.f;
-                const int ra = warp * 16 + g;
+                for (int y = 0; y < MK; ++y)
 #pragma unroll
-                for (int c = 0; c < HD / 64; ++c) {  // 16 bytes of each of the rows g and g + 8
-                    const uint32_t off = HD == 64 ? (uint32_t)(ra * 64 + ((t ^ ((ra >> 1) & 3)) << 4))
-                                                  : (uint32_t)((c >> 1) * KD_TILE * 128 + ra * 128 + (((2 * t + (c & 1)) ^ g) << 4));
-                    const uint4 ka = lds128(kb + off), kc = lds128(kb + off + 8 * LINE);
-                    const uint32_t wa[4] = {ka.x, ka.y, ka.z, ka.w}, wb[4] = {kc.x, kc.y, kc.z, kc.w};
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            acc[y][nt][e] = 0.f;
+                            if (SPLIT) low[y][nt][e] = 0.f;
+                        }
+#pragma unroll
+                for (int c = 0; c < HD / 64; ++c) {  // 16 bytes of each of the rows g and g + 8 of every block
+                    const uint32_t off = HD == 64 ? (uint32_t)(g * 64 + ((t ^ ((g >> 1) & 3)) << 4))
+                                                  : (uint32_t)((c >> 1) * KD_TILE * 128 + g * 128 + (((2 * t + (c & 1)) ^ g) << 4));
+                    uint4 ka[MK], kc[MK];
+#pragma unroll
+                    for (int y = 0; y < MK; ++y) {
+                        ka[y] = lds128(kb + off + y * 16 * LINE);
+                        kc[y] = lds128(kb + off + (y * 16 + 8) * LINE);
+                    }
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
                         const int j = HD == 64 ? w : (c >> 1) * 8 + (c & 1) * 4 + w;
-                        const uint32_t xa = kd_bias<FMT>(wa[w]), xb = kd_bias<FMT>(wb[w]);
-                        const uint32_t a0 = kd_half2<FMT>(xa, false), a1 = kd_half2<FMT>(xb, false);
-                        const uint32_t a2 = kd_half2<FMT>(xa, true), a3 = kd_half2<FMT>(xb, true);
+                        uint2 bq[NT], bl[NT];
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            const uint2 b = s_q[((nt * (SPLIT ? 2 : 1)) * KS + j) * 32 + lane];
-                            kd_mma(acc[nt][SPLIT ? 0 : w & 1], a0, a1, a2, a3, b.x, b.y);
-                            if (SPLIT) {
-                                const uint2 bl = s_q[((nt * 2 + 1) * KS + j) * 32 + lane];
-                                kd_mma(acc[nt][1], a0, a1, a2, a3, bl.x, bl.y);
+                            bq[nt] = s_q[((nt * (SPLIT ? 2 : 1)) * KS + j) * 32 + lane];
+                            if (SPLIT) bl[nt] = s_q[((nt * 2 + 1) * KS + j) * 32 + lane];
+                        }
+#pragma unroll
+                        for (int y = 0; y < MK; ++y) {
+                            const uint32_t xa = kd_bias<FMT>(w == 0 ? ka[y].x : w == 1 ? ka[y].y : w == 2 ? ka[y].z : ka[y].w);
+                            const uint32_t xb = kd_bias<FMT>(w == 0 ? kc[y].x : w == 1 ? kc[y].y : w == 2 ? kc[y].z : kc[y].w);
+                            const uint32_t a0 = kd_half2<FMT>(xa, false), a1 = kd_half2<FMT>(xb, false);
+                            const uint32_t a2 = kd_half2<FMT>(xa, true), a3 = kd_half2<FMT>(xb, true);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                kd_mma(acc[y][nt], a0, a1, a2, a3, bq[nt].x, bq[nt].y);
+                                if (SPLIT) kd_mma(low[y][nt], a0, a1, a2, a3, bl[nt].x, bl[nt].y);
                             }
                         }
                     }
                 }
                 // ---- scale, mask, the largest of each row
-                const bool masked = key0 + 15 > lim_first || (a.window > 0 && key0 < all_lo);
-                float p[NT][4];
-                const bool grow = sv > vref && sv < INFINITY;
+                const bool masked = key0 + KD_TILE - 1 > lim_first || (a.window > 0 && key0 < all_lo);
+                float vmax = 0.f;
+#pragma unroll
+                for (int y = 0; y < MK; ++y) {
+                    // out of every row's sight the page was not fetched, nor its scales
+                    if (masked && (key0 + y * 16 > lim_last || key0 + y * 16 + 15 < any_lo)) sv[y] = 0.f;
+                    if (sv[y] < INFINITY) vmax = fmaxf(vmax, sv[y]);
+                }
+                const bool grow = vmax > vref;
                 bool move = grow;
                 float mt[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float f = qs[nt][e & 1] * sk;
-                        float x = (acc[nt][0][e] + acc[nt][1][e]) * f;
-                        if (masked) {
-                            const int key = key0 + g + (e >> 1) * 8, li = lim[nt][e & 1];
-                            if (key > li || (a.window > 0 && key <= li - a.window)) x = -INFINITY;
+                    for (int y = 0; y < MK; ++y)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float x = acc[y][nt][e];
+                            if (SPLIT) x += low[y][nt][e];
+                            acc[y][nt][e] = x * (qs[nt][e & 1] * sk[y]);
                         }
-                        p[nt][e] = x;
+                    if (masked) {
+#pragma unroll
+                        for (int y = 0; y < MK; ++y)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = key0 + y * 16 + g + (e >> 1) * 8, li = lim[nt][e & 1];
+                                if (key > li || (a.window > 0 && key <= li - a.window)) acc[y][nt][e] = -INFINITY;
+                            }
                     }
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float x = fmaxf(p[nt][e], p[nt][e + 2]);
+                        float x = fmaxf(acc[0][nt][e], acc[0][nt][e + 2]);
+#pragma unroll
+                        for (int y = 1; y < MK; ++y) x = fmaxf(x, fmaxf(acc[y][nt][e], acc[y][nt][e + 2]));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                         x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -428,9 +464,9 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                 if (__any_sync(0xffffffffu, move)) {
                     float vf = 1.f;
                     if (grow) {
-                        vinv = 1.f / sv;
+                        vinv = 1.f / vmax;
                         vf = vref * vinv;
-                        vref = sv;
+                        vref = vmax;
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
@@ -447,75 +483,82 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                             }
                         }
                 }
-                // a NaN or infinite scale gives NaN to whoever sees the key
-                const float fv = !(sv < INFINITY) ? __uint_as_float(0x7fffffffu) : vref > 0.f ? sv * vinv : 1.f;
-                uint32_t b0[NT], b1[NT], c0[NT], c1[NT];
+                // ---- the weights as B fragments, with the V scale over its reference
+                uint32_t b0[MK][NT], b1[MK][NT], c0[SPLIT ? MK : 1][NT], c1[SPLIT ? MK : 1][NT];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
+                for (int y = 0; y < MK; ++y) {
+                    // a NaN or infinite scale gives NaN to whoever sees the key
+                    const float fv = !(sv[y] < INFINITY) ? __uint_as_float(0x7fffffffu) : vref > 0.f ? sv[y] * vinv : 1.f;
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float mm = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-                        const float x = kd_exp2(p[nt][e] - mm);
-                        l[nt][e & 1] += x;
-                        p[nt][e] = masked && p[nt][e] == -INFINITY ? 0.f : x * fv;
-                    }
-                    const uint32_t h0 = kd_pack(p[nt][0], p[nt][1]), h1 = kd_pack(p[nt][2], p[nt][3]);
-                    b0[nt] = kd_transpose(h0);
-                    b1[nt] = kd_transpose(h1);
-                    if (SPLIT) {
-                        c0[nt] = kd_transpose(kd_pack_rest(p[nt][0], p[nt][1], h0));
-                        c1[nt] = kd_transpose(kd_pack_rest(p[nt][2], p[nt][3], h1));
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float p[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float mm = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
+                            const float x = kd_exp2(acc[y][nt][e] - mm);
+                            l[nt][e & 1] += x;
+                            p[e] = x * fv;
+                            if (masked && acc[y][nt][e] == -INFINITY) p[e] = 0.f;
+                        }
+                        const uint32_t h0 = kd_pack(p[0], p[1]), h1 = kd_pack(p[2], p[3]);
+                        b0[y][nt] = kd_transpose(h0);
+                        b1[y][nt] = kd_transpose(h1);
+                        if (SPLIT) {
+                            c0[y][nt] = kd_transpose(kd_pack_rest(p[0], p[1], h0));
+                            c1[y][nt] = kd_transpose(kd_pack_rest(p[2], p[3], h1));
+                        }
                     }
                 }
                 // ---- O^T += V^T P^T; keys that no row sees count as zero, whatever their codes are
-                const int rv = warp * 16 + 2 * t;
-                uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
-                if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int key = key0 + 2 * t + (e & 1) + (e >> 1) * 8;
-                        keep[e] = key <= lim_last && key >= any_lo ? ~0u : 0u;
-                    }
-                }
+                for (int y = 0; y < MK; ++y) {
+                    const int rv = y * 16 + 2 * t;
 #pragma unroll
-                for (int x = 0; x < HALVES; ++x) {
-                    constexpr int WORDS = HD == 64 ? 2 : 4;
-                    uint32_t w[4][4];
+                    for (int x = 0; x < HALVES; ++x) {
+                        constexpr int WORDS = HD == 64 ? 2 : 4;
+                        uint32_t w[4][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int row = rv + (e & 1) + (e >> 1) * 8;
-                        if (HD == 64) {
-                            const uint2 v = kd_lds64(vb + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + ((g & 1) << 3));
-                            w[e][0] = v.x, w[e][1] = v.y;
-                        } else {
-                            const uint4 v = lds128(vb + x * KD_TILE * 128 + row * 128 + ((g ^ (row & 7)) << 4));
-                            w[e][0] = v.x, w[e][1] = v.y, w[e][2] = v.z, w[e][3] = v.w;
+                        for (int e = 0; e < 4; ++e) {
+                            const int row = rv + (e & 1) + (e >> 1) * 8;
+                            if (HD == 64) {
+                                const uint2 v = kd_lds64(vb + row * 64 + (((g >> 1) ^ ((row >> 1) & 3)) << 4) + ((g & 1) << 3));
+                                w[e][0] = v.x, w[e][1] = v.y;
+                            } else {
+                                const uint4 v = lds128(vb + x * KD_TILE * 128 + row * 128 + ((g ^ (row & 7)) << 4));
+                                w[e][0] = v.x, w[e][1] = v.y, w[e][2] = v.z, w[e][3] = v.w;
+                            }
                         }
                         if (masked) {
 #pragma unroll
-                            for (int k = 0; k < WORDS; ++k) w[e][k] &= keep[e];
+                            for (int e = 0; e < 4; ++e) {
+                                const int key = key0 + rv + (e & 1) + (e >> 1) * 8;
+                                if (key > lim_last || key < any_lo) {
+#pragma unroll
+                                    for (int k = 0; k < WORDS; ++k) w[e][k] = 0;
+                                }
+                            }
                         }
-                    }
 #pragma unroll
-                    for (int k = 0; k < WORDS; ++k) {
+                        for (int k = 0; k < WORDS; ++k) {
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {  // bytes 0, 1 or 2, 3 of the word: two channels
-                            const uint32_t sel = y ? 0x7362 : 0x5140;
-                            const uint32_t u = kd_bias<FMT>(__byte_perm(w[0][k], w[1][k], sel));
-                            const uint32_t v = kd_bias<FMT>(__byte_perm(w[2][k], w[3][k], sel));
-                            const uint32_t a0 = kd_half2<FMT>(u, false), a1 = kd_half2<FMT>(u, true);
-                            const uint32_t a2 = kd_half2<FMT>(v, false), a3 = kd_half2<FMT>(v, true);
-                            const int i2 = x * 8 + 2 * k + y;
+                            for (int z = 0; z < 2; ++z) {  // bytes 0, 1 or 2, 3 of the word: two channels
+                                const uint32_t sel = z ? 0x7362 : 0x5140;
+                                const uint32_t u = kd_bias<FMT>(__byte_perm(w[0][k], w[1][k], sel));
+                                const uint32_t v = kd_bias<FMT>(__byte_perm(w[2][k], w[3][k], sel));
+                                const uint32_t a0 = kd_half2<FMT>(u, false), a1 = kd_half2<FMT>(u, true);
+                                const uint32_t a2 = kd_half2<FMT>(v, false), a3 = kd_half2<FMT>(v, true);
+                                const int i2 = x * 8 + 2 * k + z;
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                if (SPLIT) {
-                                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                                    kd_mma(d, a0, a1, a2, a3, c0[nt], c1[nt]);
-                                    kd_mma(d, a0, a1, a2, a3, b0[nt], b1[nt]);
+                                for (int nt = 0; nt < NT; ++nt) {
+                                    if (SPLIT) {
+                                        float d[4] = {0.f, 0.f, 0.f, 0.f};
+                                        kd_mma(d, a0, a1, a2, a3, c0[y][nt], c1[y][nt]);
+                                        kd_mma(d, a0, a1, a2, a3, b0[y][nt], b1[y][nt]);
 #pragma unroll
-                                    for (int e = 0; e < 4; ++e) o[i2][nt][e] += d[e];
-                                } else {
-                                    kd_mma(o[i2][nt], a0, a1, a2, a3, b0[nt], b1[nt]);
+                                        for (int e = 0; e < 4; ++e) o[i2][nt][e] += d[e];
+                                    } else {
+                                        kd_mma(o[i2][nt], a0, a1, a2, a3, b0[y][nt], b1[y][nt]);
+                                    }
                                 }
                             }
                         }
@@ -525,6 +568,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[s]);
         }
+        it += cnt;
         // ---- the four warps' results into one: largest m, then sum of o * v_ref * 2^(m - M)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
