@@ -27,6 +27,12 @@ __device__ __forceinline__ uint32_t kv8_code(float y) {
     }
     return y != y ? 0u : (uint32_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }
+// Codes of two values, the first in the low byte.
+template <int FMT>
+__device__ __forceinline__ uint32_t kv8_code2(float a, float b) {
+    if (FMT == KV8_INT8) return kv8_code<FMT>(a) | (kv8_code<FMT>(b) << 8);
+    return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a != a ? 0.f : a, b != b ? 0.f : b), __NV_SATFINITE, __NV_E4M3);
+}
 template <int FMT>
 __device__ __forceinline__ float kv8_value(uint32_t code) {
     if (FMT == KV8_INT8) return (float)(int8_t)code;
@@ -34,6 +40,21 @@ __device__ __forceinline__ float kv8_value(uint32_t code) {
     const uint32_t h = ((code & 0x80u) << 8) | ((code & 0x7fu) << 7);
     return half_bits_to_float(h) * 256.f;
 }
+
+// two codes (bytes lo and lo + 1 of w) -> two fp16, exactly
+template <int FMT>
+__device__ __forceinline__ uint32_t kd_half2(uint32_t w, bool high) {
+    if (FMT == KV8_INT8) {
+        // w holds code + 128: bytes beside 0x64 are the fp16 numbers 1024 + byte; less 1152
+        const uint32_t x = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
+        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? w >> 16 : w & 0xffffu), __NV_E4M3);
+    return (uint32_t)r.x | ((uint32_t)r.y << 16);
+}
+template <int FMT>
+__device__ __forceinline__ uint32_t kd_bias(uint32_t w) { return FMT == KV8_INT8 ? w ^ 0x80808080u : w; }
 
 // 8 consecutive elements of a row of activations. `wide`: the row is 16-byte aligned.
 __device__ __forceinline__ void kv8_ld8(const void* base, long long i, int type, bool wide, float (&x)[8]) {
@@ -67,6 +88,37 @@ __device__ __forceinline__ void kv8_ld8(const void* base, long long i, int type,
             x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
         }
     }
+}
+// The same with the type known: 16 raw bytes per 8 elements of 16 bits, 32 per 8 floats, and their values.
+template <int TYPE, bool WIDE>
+__device__ __forceinline__ void kv8_raw8(const void* base, long long i, uint32_t (&w)[TYPE == FENCE_F32 ? 8 : 4]) {
+    if (TYPE == FENCE_F32) {
+        const uint32_t* p = static_cast<const uint32_t*>(base) + i;
+        if (WIDE) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p), b = *reinterpret_cast<const uint4*>(p + 4);
+            constexpr int O = TYPE == FENCE_F32 ? 4 : 0;
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[O] = b.x, w[O + 1] = b.y, w[O + 2] = b.z, w[O + 3] = b.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < (TYPE == FENCE_F32 ? 8 : 4); ++j) w[j] = p[j];
+        }
+    } else {
+        const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+        if (WIDE) {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = (uint32_t)p[2 * j] | ((uint32_t)p[2 * j + 1] << 16);
+        }
+    }
+}
+template <int TYPE>
+__device__ __forceinline__ float kv8_elem(const uint32_t (&w)[TYPE == FENCE_F32 ? 8 : 4], int j) {  // j a constant
+    if (TYPE == FENCE_F32) return __uint_as_float(w[TYPE == FENCE_F32 ? j : 0]);
+    const uint32_t x = w[TYPE == FENCE_F32 ? 0 : j >> 1];
+    if (TYPE == FENCE_F16) return half_bits_to_float(j & 1 ? x >> 16 : x);
+    return __uint_as_float(j & 1 ? x & 0xffff0000u : x << 16);
 }
 __device__ __forceinline__ uint32_t kv8_pack2(float a, float b, int type) {
     if (type == FENCE_F16) {

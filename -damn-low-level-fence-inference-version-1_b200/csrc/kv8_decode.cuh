@@ -73,21 +73,6 @@ struct KDShape {
     static constexpr int SMEM = O_SCAN + 64 + 1024;  // + the prefix sums [n_req + 1], + alignment
 };
 
-// two codes (bytes lo and lo + 1 of w) -> two fp16, exactly
-template <int FMT>
-__device__ __forceinline__ uint32_t kd_half2(uint32_t w, bool high) {
-    if (FMT == KV8_INT8) {
-        // w holds code + 128: bytes beside 0x64 are the fp16 numbers 1024 + byte; less 1152
-        const uint32_t x = __byte_perm(w, 0x64646464u, high ? 0x4342 : 0x4140);
-        const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-        return *reinterpret_cast<const uint32_t*>(&h);
-    }
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? w >> 16 : w & 0xffffu), __NV_E4M3);
-    return (uint32_t)r.x | ((uint32_t)r.y << 16);
-}
-template <int FMT>
-__device__ __forceinline__ uint32_t kd_bias(uint32_t w) { return FMT == KV8_INT8 ? w ^ 0x80808080u : w; }
-
 __device__ __forceinline__ void kd_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
     asm volatile(
