@@ -160,6 +160,23 @@ __device__ __forceinline__ void kv8_st1(void* base, long long i, int type, float
     else static_cast<__nv_bfloat16*>(base)[i] = __float2bfloat16_rn(x);
 }
 
+// Launches with programmatic stream serialization: the kernel's launch and set-up overlap the end of the kernel before it.
+// Every kernel launched so waits for that one (pdl_wait) before it touches global memory, so the order is the stream's.
+template <typename... P, typename... A>
+inline cudaError_t kv8_launch(void (*kern)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
 inline int kv8_elem_size(int type) { return type == FENCE_F32 ? 4 : 2; }
 // whether every row of a [rows][stride] buffer that starts at a multiple of 8 elements is 16-byte aligned
 inline bool kv8_wide(const void* p, long long stride, int type) {

@@ -46,8 +46,8 @@ static int kv8_launch_decode(const KAttnArgs& p, cudaStream_t st) {
     auto kern = kv8_decode_kernel<FMT, HD, SPLIT, NT>;
     FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM + 4 * (FENCE_PAGED_MAX_REQ + 1), done));
     const int smem = S::SMEM + 4 * (p.n_req + 1), fit = 228 * 1024 / (smem + 1024);  // many requests' prefix sums can cost a CTA
-    kern<<<KV8_SMS * (fit < S::CTAS ? fit : S::CTAS), KD_THREADS, smem, st>>>(p, tm_k, tm_v);
-    return cuda_status(cudaGetLastError(), "kv8_attention");
+    const dim3 grid((unsigned)(KV8_SMS * (fit < S::CTAS ? fit : S::CTAS)));
+    return cuda_status(kv8_launch(kern, grid, KD_THREADS, smem, st, p, tm_k, tm_v), "kv8_attention");
 }
 
 template <int FMT, int HD, bool SPLIT>
@@ -61,22 +61,10 @@ static int kv8_launch_prefill(const KAttnArgs& p, cudaStream_t st) {
     const long long rows = (long long)p.n_tokens * p.n_q_heads;
     if (!tg_tensor_map(&tm_q, p.q_rows, (int)(rows * (SPLIT ? 2 : 1)), HD, 128))
         return set_error(FENCE_E_UNSUPPORTED, "kv8_attention: no tensor map for the query rows");
-    kv8_q_rows_kernel<HD, SPLIT><<<(unsigned)((rows + KQ_WARPS - 1) / KQ_WARPS), 32 * KQ_WARPS, 0, st>>>(p);
-    FENCE_CUDA_TRY(cudaGetLastError());
+    FENCE_CUDA_TRY(kv8_launch(kv8_q_rows_kernel<HD, SPLIT>, dim3((unsigned)((rows + KQ_WARPS - 1) / KQ_WARPS)), 32 * KQ_WARPS, 0, st, p));
     auto kern = kv8_prefill_kernel<FMT, HD, SPLIT>;
     FENCE_CUDA_TRY(kv8_opt_in(kern, S::SMEM, done));
-    // its set-up runs beside the q rows' kernel; it waits for that one before it reads them
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(KP_SMS);
-    cfg.blockDim = dim3(KP_THREADS);
-    cfg.dynamicSmemBytes = S::SMEM;
-    cfg.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, kern, p, tm_q, tm_k, tm_v), "kv8_attention");
+    return cuda_status(kv8_launch(kern, dim3(KP_SMS), KP_THREADS, S::SMEM, st, p, tm_q, tm_k, tm_v), "kv8_attention");
 }
 
 constexpr size_t KV8_ARRIVED_BYTES = 4096;  // counters, at the workspace's start: 2048 for each kernel
@@ -114,6 +102,7 @@ static int kv8_launch_attn(const KAttnArgs& pd, bool split, int nt, bool prefill
             const int e = split ? kv8_launch_prefill<FMT, HD, true>(p, st) : kv8_launch_prefill<FMT, HD, false>(p, st);
             if (e || p.n_req == 1) return e;
             p.max_rows = KV8_DECODE_ROWS;
+            p.behind_prefill = 1;
             p.arrived = pd.arrived;
             p.part = pd.part;
         }
@@ -168,7 +157,7 @@ extern "C" int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_b
         return set_error(FENCE_E_SCRATCH, "kv8_attention: workspace of %zu bytes, needs %zu", a->workspace_bytes, need);
     KAttnArgs p{*c, b->block_table, b->kv_len, b->new_start, b->n_req, b->n_tokens, b->max_pages, ilog2(c->page_tokens),
                 a->n_q_heads / c->n_kv_heads, a->n_q_heads, a->window > 0 ? a->window : 0, a->type, a->q, a->out, a->lse,
-                a->q_stride, a->out_stride, (float)(a->scale * 1.4426950408889634), INT_MAX, 0, kv8_wide(a->q, a->q_stride, a->type),
+                a->q_stride, a->out_stride, (float)(a->scale * 1.4426950408889634), INT_MAX, 0, 0, kv8_wide(a->q, a->q_stride, a->type),
                 kv8_wide(a->out, a->out_stride, a->type), nullptr, nullptr, static_cast<int*>(a->workspace),
                 reinterpret_cast<float*>(static_cast<char*>(a->workspace) + KV8_ARRIVED_BYTES)};
     const bool split = a->type == FENCE_F32, prefill = kv8_has_prefill(c, a);

@@ -40,6 +40,7 @@ struct KAttnArgs {
     long long q_stride, out_stride;
     float scale_log2;  // scale * log2(e): scores are kept as exponents of 2
     int max_rows;      // decode kernel: requests of more query rows per KV head are left to the prefill kernel
+    int behind_prefill;    // decode kernel: the kernel before is this call's prefill kernel, with other rows: no need to wait for it
     int min_rows;      // prefill kernel: requests of at most this many are the decode kernel's
     int q_wide, out_wide;  // rows are 16-byte aligned
     __half* q_rows;        // prefill kernel: [2][n_kv_heads][n_tokens * G][head_dim], rows of q as it multiplies them (high, low)
@@ -162,6 +163,11 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
         }
         fence_barrier_init();
     }
+    // The prefill kernel of the same call lets this one start once it has itself waited for all before it.
+    if (!a.behind_prefill) {
+        pdl_launch_dependents();
+        pdl_wait();
+    }
     // ---- prefix sums of the requests' tiles
     {
         const int per = (a.n_req + KD_THREADS - 1) / KD_THREADS;
@@ -264,6 +270,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
             cur = unit0 + KD_UNIT + first + cnt;
         }
         cp_async_wait_all();
+        if (a.behind_prefill) pdl_wait();  // so that what comes next waits for both
         return;
     }
     // -------------------------------------------------------------------- consumers
@@ -685,6 +692,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
         named_bar_sync(1, 32 * KD_WARPS);
         cur = unit0 + KD_UNIT + first + cnt;
     }
+    if (a.behind_prefill) pdl_wait();
 }
 
 }  // namespace fence

@@ -58,6 +58,7 @@ constexpr int KQ_WARPS = 8;
 template <int HD, bool SPLIT>
 __global__ void __launch_bounds__(32 * KQ_WARPS) kv8_q_rows_kernel(const KAttnArgs a) {
     pdl_launch_dependents();
+    pdl_wait();
     constexpr int EPL = HD / 32;
     const int lane = threadIdx.x & 31;
     const long long i = (long long)blockIdx.x * KQ_WARPS + (threadIdx.x >> 5), per_head = (long long)a.n_tokens * a.G;
@@ -353,6 +354,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_misc)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // The q rows' kernel lets this one start while it waits itself for what came before: all of that has to be done here too.
+    pdl_wait();
+    pdl_launch_dependents();
     // ---- where this CTA's run begins: prefix sums over the requests, in the space of the operands
     KPWalk<ROWS> walk;
     walk.lane = lane;
@@ -489,7 +493,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         // ---------------------------------------------------------------- codes into the stages
         const int box = min(a.c.page_tokens, 64), boxes = KP_KT / box;
         uint32_t it = 0, segs = 0;
-        pdl_wait();  // q's rows come from the kernel before
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
             bool q_due = true;
@@ -666,7 +669,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         const int s = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16), t_s = t_lane + 128 * s, t_o = t_lane + 256 + 128 * s;
         uint32_t n_s = 0, n_o = 0, it = 0;
-        pdl_wait();
         // rows that belong to no request
         if (a.min_rows == 0) {
             const int used = max(0, min(a.new_start[a.n_req], a.n_tokens));

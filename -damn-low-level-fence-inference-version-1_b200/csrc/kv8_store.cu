@@ -21,6 +21,8 @@ constexpr int KV8_ST_CHUNKS = 8;  // of 8 elements, at most, per thread: a page 
 // loops, 8000 rows of 8 x 128 bf16 took 23 us against 7.6 us of traffic). Threads: the page's elements / 64, 128 to 512.
 template <int FMT, int TYPE, bool WIDE>
 __global__ void __launch_bounds__(512) kv8_store_kernel(const StoreArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int4 e = a.touch[blockIdx.x];  // page, first row, first token, rows
     if (e.x < 0) return;
     const int P = a.c.page_tokens, hd = a.c.head_dim, h = blockIdx.y, kv = blockIdx.z, cpr = hd / 8, shift = 31 - __clz(cpr);
@@ -98,6 +100,8 @@ struct LoadArgs {
 constexpr int KV8_LD_ITEMS = 2;
 template <int FMT>
 __global__ void __launch_bounds__(256) kv8_load_kernel(const LoadArgs a) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int hd = a.c.head_dim, cpr = hd / 16, row = a.c.n_kv_heads * cpr, kv = blockIdx.y, shift = 31 - __clz(cpr);
     if (!a.x[kv]) return;
     const uint8_t* codes = static_cast<const uint8_t*>(kv ? a.c.v : a.c.k);
@@ -148,15 +152,15 @@ __global__ void __launch_bounds__(256) kv8_load_kernel(const LoadArgs a) {
 }
 
 template <int FMT, int TYPE>
-static void kv8_launch_store(const StoreArgs& a, dim3 grid, int threads, cudaStream_t st) {
-    if (a.wide[0] && a.wide[1]) kv8_store_kernel<FMT, TYPE, true><<<grid, threads, 0, st>>>(a);
-    else kv8_store_kernel<FMT, TYPE, false><<<grid, threads, 0, st>>>(a);
+static cudaError_t kv8_launch_store(const StoreArgs& a, dim3 grid, int threads, cudaStream_t st) {
+    if (a.wide[0] && a.wide[1]) return kv8_launch(kv8_store_kernel<FMT, TYPE, true>, grid, threads, 0, st, a);
+    return kv8_launch(kv8_store_kernel<FMT, TYPE, false>, grid, threads, 0, st, a);
 }
 template <int FMT>
-static void kv8_launch_store(const StoreArgs& a, dim3 grid, int threads, cudaStream_t st) {
-    if (a.type == FENCE_F32) kv8_launch_store<FMT, FENCE_F32>(a, grid, threads, st);
-    else if (a.type == FENCE_F16) kv8_launch_store<FMT, FENCE_F16>(a, grid, threads, st);
-    else kv8_launch_store<FMT, FENCE_BF16>(a, grid, threads, st);
+static cudaError_t kv8_launch_store(const StoreArgs& a, dim3 grid, int threads, cudaStream_t st) {
+    if (a.type == FENCE_F32) return kv8_launch_store<FMT, FENCE_F32>(a, grid, threads, st);
+    if (a.type == FENCE_F16) return kv8_launch_store<FMT, FENCE_F16>(a, grid, threads, st);
+    return kv8_launch_store<FMT, FENCE_BF16>(a, grid, threads, st);
 }
 
 }  // namespace fence
@@ -183,9 +187,10 @@ extern "C" int fence_kv8_store(const fence_kv8_cache* c, const fence_paged_batch
     const dim3 grid((unsigned)b->n_touch, (unsigned)c->n_kv_heads, 2);
     int threads = c->page_tokens * c->head_dim / (8 * KV8_ST_CHUNKS);
     threads = threads < 128 ? 128 : threads;  // at most 128 * 256 / 64 = 512
-    if (c->format == KV8_INT8) kv8_launch_store<KV8_INT8>(a, grid, threads, (cudaStream_t)stream);
-    else kv8_launch_store<KV8_E4M3>(a, grid, threads, (cudaStream_t)stream);
-    return cuda_status(cudaGetLastError(), "kv8_store");
+    const cudaStream_t st = (cudaStream_t)stream;
+    return cuda_status(c->format == KV8_INT8 ? kv8_launch_store<KV8_INT8>(a, grid, threads, st)
+                                             : kv8_launch_store<KV8_E4M3>(a, grid, threads, st),
+                       "kv8_store");
 }
 
 extern "C" int fence_kv8_load(const fence_kv8_cache* c, const int* slot, int n, void* k, void* v, int type, long long k_stride,
@@ -207,7 +212,7 @@ extern "C" int fence_kv8_load(const fence_kv8_cache* c, const int* slot, int n, 
     const long long blocks = (items + 256 * KV8_LD_ITEMS - 1) / (256 * KV8_LD_ITEMS);
     if (blocks > INT_MAX) return set_error(FENCE_E_UNSUPPORTED, "kv8_load: %d rows", n);
     const dim3 grid((unsigned)blocks, 2);
-    if (c->format == KV8_INT8) kv8_load_kernel<KV8_INT8><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
-    else kv8_load_kernel<KV8_E4M3><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
-    return cuda_status(cudaGetLastError(), "kv8_load");
+    return cuda_status(kv8_launch(c->format == KV8_INT8 ? kv8_load_kernel<KV8_INT8> : kv8_load_kernel<KV8_E4M3>, grid, 256, 0,
+                                  (cudaStream_t)stream, a),
+                       "kv8_load");
 }

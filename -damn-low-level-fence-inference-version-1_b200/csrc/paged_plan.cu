@@ -57,6 +57,8 @@ __device__ __forceinline__ int plan_find(const int* a, int n, int v) {
 }
 
 __global__ void paged_plan_kernel(const PlanArgs p) {
+    pdl_launch_dependents();
+    pdl_wait();
     extern __shared__ int s_mem[];
     __shared__ long long s_warp[32];
     __shared__ int s_used;
@@ -258,6 +260,5 @@ extern "C" int fence_paged_plan(const fence_paged_batch* b, fence_stream_t strea
     if (smem > 48 * 1024)
         FENCE_CUDA_TRY(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             (6 * FENCE_PAGED_MAX_REQ + 4) * (int)sizeof(int)));
-    paged_plan_kernel<<<grid, threads, smem, (cudaStream_t)stream>>>(p);
-    return cuda_status(cudaGetLastError(), "paged_plan");
+    return cuda_status(kv8_launch(paged_plan_kernel, dim3((unsigned)grid), threads, smem, (cudaStream_t)stream, p), "paged_plan");
 }
