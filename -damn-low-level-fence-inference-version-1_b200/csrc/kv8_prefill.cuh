@@ -31,6 +31,9 @@ namespace fence {
 constexpr int KP_KT = 128, KP_SMS = 148;
 constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_W_LOAD = 14, KP_THREADS = 480;
 constexpr int KP_MIN_TILES = 2, KP_SLOTS = 4;
+// SPLIT: the matrix unit's additions cut the sum's last bit off, half of it on average and always towards zero: 128 of
+// them (8 tiles) cost 2e-6. So after every 4 tiles of a stream the sums are added, rounded, to the stream's record.
+constexpr int KP_DRAIN = 4;
 
 template <int HD, bool SPLIT>
 struct KPShape {
@@ -590,7 +593,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
             int pend0 = -1, pend1 = -1;      // the tile (count) whose weights a stream is making
-            uint32_t have = 0, left = 0;     // have: q (bits 0, 1) and o (2, 3) of the streams; left: streams that still need V, 8 bits per buffer
+            uint32_t have = 0, left = 0, made[2] = {0, 0};  // have: q (bits 0, 1) and o (2, 3) of the streams; left: streams that still need V, 8 bits per buffer
             const int last = g.tile0 + g.cnt;
             // one more round than tiles, two where the streams take turns, to finish the last weights
             for (int kt = g.tile0; kt < last + (SPLIT ? 2 : 1); ++kt) {
@@ -606,8 +609,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         wait(&p_full[s], np >> (16 * s));
                         np ^= 1u << (16 * s);
                         left -= 1u << (8 * pb);
-                        const uint32_t add = (have >> (2 + s)) & 1u;
+                        uint32_t add = (have >> (2 + s)) & 1u;
                         have |= 4u << s;
+                        if (SPLIT) {
+                            add = (s ? made[1] : made[0]) % KP_DRAIN != 0;
+                            if (s) ++made[1];
+                            else ++made[0];
+                        }
                         kp_fence_after();
                         const uint32_t d = __shfl_sync(0xffffffffu, tm + 256 + 128 * s, 0), ta = __shfl_sync(0xffffffffu, tm + 128 * s, 0);
                         const uint64_t db = kp_desc_mn(__shfl_sync(0xffffffffu, sbase + S::O_V + pb * S::OP, 0), KP_KT * 128);
@@ -694,6 +702,38 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const float qs = valid ? a.q_scale[(long long)g.h * a.n_tokens * a.G + tok * a.G + (g.row0 + i_row) % a.G] : 1.f;
             float m = -INFINITY, l = 0.f, lvref = -INFINITY, vref = 0.f;
             bool have_o = false;
+            // the record of (CTA, slot, stream): m and l of each row, then the sums, four channels of all rows after one another
+            auto record = [&]() { return a.part + ((long long)blockIdx.x * 4 + (g.first > 0 ? 0 : 2) + s) * S::REC; };
+            float m_rec = -INFINITY;  // SPLIT: what the record's sums so far are relative to
+            int since = 0, drained = 0;
+            auto drain = [&]() {  // the sums to the record
+                const float f = drained ? kd_exp2(m_rec - (m == -INFINITY ? 0.f : m)) : 0.f;
+                float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
+#pragma unroll 1
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t r[16];
+                    if (have_o) {
+                        KP_LD16(r, t_o + c);
+                        kp_wait_ld();
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        float4* at = rec + ((c + e) >> 2) * 128;
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (SPLIT && drained) {
+                            v = __ldcg(at);
+                            v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+                        }
+                        if (have_o) {
+                            v.x = fmaf(__uint_as_float(r[e]), vref, v.x), v.y = fmaf(__uint_as_float(r[e + 1]), vref, v.y);
+                            v.z = fmaf(__uint_as_float(r[e + 2]), vref, v.z), v.w = fmaf(__uint_as_float(r[e + 3]), vref, v.w);
+                        }
+                        __stcg(at, v);
+                    }
+                }
+                drained = 1;
+                m_rec = m;
+            };
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j, key0 = kt * KP_KT;
                 const bool act = kp_active<SPLIT>(g, s, kt);
@@ -709,6 +749,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 wait(&s_full[s], n_s++);
                 __syncwarp();
                 kp_fence_after();
+                if (SPLIT && since == KP_DRAIN) {  // the products of the tiles before have ended: S came after them
+                    drain();
+                    since = 0;
+                    have_o = false;
+                    kp_fence_before();
+                }
+                if (SPLIT) ++since;
                 const float* pr = s_prep + slot * 24;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
                 // Loops of 32 columns, not unrolled: the roles' code has to share the instruction cache.
                 const bool edge = key0 + KP_KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
@@ -845,36 +892,38 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const bool whole = g.cnt == g.tiles, direct = whole && !SPLIT;
             const int unit0 = cur - g.first;
             const int c_first = unit0 / per, c_last = (unit0 + g.tiles - 1) / per;
-            // the sums go out as they are, or to the record of (CTA, slot, stream): m and l of each row, then four channels
-            // of all rows after one another
-            float* rec = a.part + ((long long)blockIdx.x * 4 + (g.first > 0 ? 0 : 2) + s) * S::REC;
-            const float mul = direct ? (l == 0.f ? 0.f : vref / l) : vref;
+            if (SPLIT) {
+                drain();
+            } else {  // out, or to the record
+                const float mul = direct ? (l == 0.f ? 0.f : vref / l) : vref;
+                float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-                uint32_t r[16];
-                float x[16];
-                if (have_o) {
-                    KP_LD16(r, t_o + c);
-                    kp_wait_ld();
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) x[e] = have_o && mul != 0.f ? __uint_as_float(r[e]) * mul : 0.f;
-                if (direct) {
-                    const long long at = tok * a.out_stride + (long long)head * HD + c;
-                    if (valid) {
-                        kv8_st8(a.out, at, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x));
-                        kv8_st8(a.out, at + 8, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x + 8));
+                for (int c = 0; c < HD; c += 16) {
+                    uint32_t r[16];
+                    float x[16];
+                    if (have_o) {
+                        KP_LD16(r, t_o + c);
+                        kp_wait_ld();
                     }
-                } else {
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4)
-                        __stcg(reinterpret_cast<float4*>(rec + 256) + ((c + e) >> 2) * 128 + row, make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                    for (int e = 0; e < 16; ++e) x[e] = have_o && mul != 0.f ? __uint_as_float(r[e]) * mul : 0.f;
+                    if (direct) {
+                        const long long at = tok * a.out_stride + (long long)head * HD + c;
+                        if (valid) {
+                            kv8_st8(a.out, at, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x));
+                            kv8_st8(a.out, at + 8, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x + 8));
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4)
+                            __stcg(rec + ((c + e) >> 2) * 128, make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                    }
                 }
             }
             if (direct) {
                 if (valid && a.lse) a.lse[tok * a.n_q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
             } else {
-                __stcg(reinterpret_cast<float2*>(rec) + row, make_float2(m, l));
+                __stcg(reinterpret_cast<float2*>(record()) + row, make_float2(m, l));
                 __threadfence();
                 named_bar_sync(1, 256);
                 if (tid == 0) {
