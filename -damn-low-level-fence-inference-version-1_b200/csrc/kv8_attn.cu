@@ -72,11 +72,12 @@ constexpr int KV8_DECODE_ROWS = 16;         // the most query rows per KV head o
 
 // Whether the batch needs the prefill kernel.
 static bool kv8_has_prefill(const fence_kv8_cache* c, const fence_kv8_attn* a) {
-    return c->head_dim <= 128 && (long long)a->max_new * (a->n_q_heads / c->n_kv_heads) > KV8_DECODE_ROWS;
+    // 256 channels of fp32 queries, as pairs, leave no room for the keys there
+    return (c->head_dim <= 128 || a->type != FENCE_F32) && (long long)a->max_new * (a->n_q_heads / c->n_kv_heads) > KV8_DECODE_ROWS;
 }
 // The workspace: counters, the decode kernel's partial results, the prefill kernel's, its query rows and their scales.
 static size_t kv8_prefill_part_bytes(const fence_kv8_cache* c) {
-    return (size_t)KP_SMS * 4 * 128 * (c->head_dim + 2) * sizeof(float);
+    return (size_t)KP_SMS * 4 * 128 * ((c->head_dim < 128 ? c->head_dim : 128) + 2) * sizeof(float);
 }
 static size_t kv8_q_rows_bytes(const fence_kv8_cache* c, const fence_paged_batch* b, const fence_kv8_attn* a) {
     return ((size_t)b->n_tokens * a->n_q_heads * c->head_dim * 2 * (a->type == FENCE_F32 ? 2 : 1) + 255) & ~(size_t)255;
@@ -89,23 +90,23 @@ template <int FMT, int HD>
 static int kv8_launch_attn(const KAttnArgs& pd, bool split, int nt, bool prefill, char* ws, size_t q_bytes,
                            cudaStream_t st) {
     KAttnArgs p = pd;
-    if constexpr (HD <= 128) {
-        if (prefill) {
-            // one request: the prefill kernel takes it whatever its length is
-            p.min_rows = p.n_req == 1 ? 0 : KV8_DECODE_ROWS;
-            p.arrived = reinterpret_cast<int*>(ws + 2048);
-            char* at = ws + KV8_ARRIVED_BYTES + kv8_decode_part_bytes(&p.c);
-            p.part = reinterpret_cast<float*>(at);
-            at += kv8_prefill_part_bytes(&p.c);
-            p.q_rows = reinterpret_cast<__half*>(at);
-            p.q_scale = reinterpret_cast<float*>(at + q_bytes);
-            const int e = split ? kv8_launch_prefill<FMT, HD, true>(p, st) : kv8_launch_prefill<FMT, HD, false>(p, st);
-            if (e || p.n_req == 1) return e;
-            p.max_rows = KV8_DECODE_ROWS;
-            p.behind_prefill = 1;
-            p.arrived = pd.arrived;
-            p.part = pd.part;
-        }
+    if (prefill) {
+        // one request: the prefill kernel takes it whatever its length is
+        p.min_rows = p.n_req == 1 ? 0 : KV8_DECODE_ROWS;
+        p.arrived = reinterpret_cast<int*>(ws + 2048);
+        char* at = ws + KV8_ARRIVED_BYTES + kv8_decode_part_bytes(&p.c);
+        p.part = reinterpret_cast<float*>(at);
+        at += kv8_prefill_part_bytes(&p.c);
+        p.q_rows = reinterpret_cast<__half*>(at);
+        p.q_scale = reinterpret_cast<float*>(at + q_bytes);
+        int e;
+        if constexpr (HD <= 128) e = split ? kv8_launch_prefill<FMT, HD, true>(p, st) : kv8_launch_prefill<FMT, HD, false>(p, st);
+        else e = kv8_launch_prefill<FMT, HD, false>(p, st);
+        if (e || p.n_req == 1) return e;
+        p.max_rows = KV8_DECODE_ROWS;
+        p.behind_prefill = 1;
+        p.arrived = pd.arrived;
+        p.part = pd.part;
     }
     if (split) return nt == 1 ? kv8_launch_decode<FMT, HD, true, 1>(p, st) : kv8_launch_decode<FMT, HD, true, 2>(p, st);
     return nt == 1 ? kv8_launch_decode<FMT, HD, false, 1>(p, st) : kv8_launch_decode<FMT, HD, false, 2>(p, st);

@@ -12,7 +12,8 @@
 //  * Rows of a group are (token, query head of the KV head): grouped heads share every K and V tile.
 //    Two streams of 128 rows per CTA take turns on the matrix unit: while one stream's softmax warps
 //    work, the other's products run. fp32 activations (SPLIT): one group of 128 rows, q and the weights as
-//    pairs of fp16, and the two streams take the even and the odd tiles.
+////    pairs of fp16, and the two streams take the even and the odd tiles. head_dim 256: both take every tile of
+//    64 keys, and half the output channels (the scores are made twice: the sums of 256 channels fill two streams' space).
 //  * Codes become fp16 exactly, once per tile for both streams, by four converter warps, from stages that
 //    TMA fills a tile ahead, and stored as they lie, keys by channels, in 128-byte swizzled shared
 //    memory: a K-major operand for S, an MN-major one for O. Scales never touch the codes: k_scale is
@@ -28,7 +29,7 @@
 
 namespace fence {
 
-constexpr int KP_KT = 128, KP_SMS = 148;
+constexpr int KP_SMS = 148;
 constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_W_LOAD = 14, KP_THREADS = 480;
 constexpr int KP_MIN_TILES = 2, KP_SLOTS = 4;
 // SPLIT: the matrix unit's additions cut the sum's last bit off, half of it on average and always towards zero: 128 of
@@ -37,19 +38,23 @@ constexpr int KP_DRAIN = 4;
 
 template <int HD, bool SPLIT>
 struct KPShape {
-    static constexpr int ROWS = SPLIT ? 128 : 256;  // per group
+    static_assert(HD <= 128 || !SPLIT, "two parts of 256 channels of q leave no room for the keys");
+    static constexpr bool HALVES = HD == 256;       // the streams share rows and tiles and take 128 output channels each
+    static constexpr int KT = HALVES ? 64 : 128;    // keys per tile
+    static constexpr int HDO = HALVES ? 128 : HD;   // channels of a stream's sums
+    static constexpr int ROWS = SPLIT || HALVES ? 128 : 256;  // per group
     static constexpr int Q_TILE = 128 * HD * 2;     // 128 rows as fp16
-    static constexpr int OP = KP_KT * HD * 2;       // a K or V operand tile
-    static constexpr int O_Q = 0;  // two tiles: the streams' rows, or the high and low parts
-    static constexpr int O_K = 2 * Q_TILE;
+    static constexpr int OP = KT * HD * 2;          // a K or V operand tile
+    static constexpr int O_Q = 0;  // two tiles: the streams' rows, or the high and low parts; one where the rows are shared
+    static constexpr int O_K = (HALVES ? 1 : 2) * Q_TILE;
     static constexpr int O_V = O_K + 2 * OP;
-    static constexpr int RAW = KP_KT * HD;          // staged codes of a K or V tile
+    static constexpr int RAW = KT * HD;             // staged codes of a K or V tile
     static constexpr int O_RAW = O_V + 2 * OP;
     static constexpr int O_BAR = O_RAW + 2 * RAW;
     static constexpr int O_MISC = O_BAR + 256;
     static constexpr int O_PREP = O_MISC + 64;  // [KP_SLOTS][24]: k_scale, log2 v_scale, 1 / v_scale of 8 x 16 keys; [KP_SLOTS][8]: the pool's row of their first
     static constexpr int SMEM = O_PREP + KP_SLOTS * 128 + 1024;
-    static constexpr int REC = 128 * (HD + 2);  // floats of one stream's partial result
+    static constexpr int REC = 128 * (HDO + 2);  // floats of one stream's partial result
 };
 
 // The rows of q as the prefill kernel multiplies them, in its order (KV head, token, query head of the KV head): by a power of
@@ -84,6 +89,9 @@ __global__ void __launch_bounds__(32 * KQ_WARPS) kv8_q_rows_kernel(const KAttnAr
         if (a.q_wide && EPL == 4) {
             const uint2 v = *reinterpret_cast<const uint2*>(p);
             w[0] = v.x, w[EPL / 2 - 1] = v.y;
+        } else if (a.q_wide && EPL == 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p);
+            w[0] = v.x, w[1 % (EPL / 2)] = v.y, w[2 % (EPL / 2)] = v.z, w[3 % (EPL / 2)] = v.w;
         } else {
 #pragma unroll
             for (int e = 0; e < EPL / 2; ++e) w[e] = (uint32_t)p[2 * e] | ((uint32_t)p[2 * e + 1] << 16);
@@ -127,16 +135,17 @@ struct KPSeg {
     int lo[2], hi[2];                              // the tiles that rows of each stream see
 };
 
+template <int KT>
 __device__ __forceinline__ void kp_group(const KAttnArgs& a, const KReq& q, int rows_per_group, int gi, int* lo_tile, int* tiles) {
     const int nrows = q.n * a.G, r_lo = gi * rows_per_group, r_hi = min(r_lo + rows_per_group, nrows) - 1;
     const int first = q.kv - q.n + r_lo / a.G, last = q.kv - q.n + r_hi / a.G;
     const int lo = a.window > 0 ? max(0, first - a.window + 1) : 0;
-    *lo_tile = last < 0 ? 0 : lo / KP_KT;
-    *tiles = last < 0 ? 1 : last / KP_KT - *lo_tile + 1;
+    *lo_tile = last < 0 ? 0 : lo / KT;
+    *tiles = last < 0 ? 1 : last / KT - *lo_tile + 1;
 }
 
 // Walks a CTA's run of tiles; every warp does so for itself, all lanes together.
-template <int ROWS>
+template <int ROWS, int KT>
 struct KPWalk {
     int r, base, per_head;  // request, tiles before it, tiles of one of its heads
     KReq q;
@@ -145,7 +154,7 @@ struct KPWalk {
         int sum = 0;
         for (int g0 = 0; g0 < x.groups; g0 += 32) {
             int lo, t = 0;
-            if (g0 + lane < x.groups) kp_group(a, x, ROWS, g0 + lane, &lo, &t);
+            if (g0 + lane < x.groups) kp_group<KT>(a, x, ROWS, g0 + lane, &lo, &t);
             sum += __reduce_add_sync(0xffffffffu, (unsigned)t);
         }
         return sum;
@@ -155,7 +164,7 @@ struct KPWalk {
     }
     __device__ __forceinline__ void enter(const KAttnArgs& a, int request, int before) {
         r = request, base = before;
-        q = kd_request(a, r, ROWS, KP_KT, false);
+        q = kd_request(a, r, ROWS, KT, false);
         per_head = mine(a, q) ? count(a, q) : 0;
     }
     // to the tile `cur` of the list, cur < total
@@ -165,7 +174,7 @@ struct KPWalk {
             int next = r + 1;
             for (;;) {  // the next request of this kernel, 32 at a time
                 bool m = false;
-                if (next + lane < a.n_req) m = mine(a, kd_request(a, next + lane, ROWS, KP_KT, false));
+                if (next + lane < a.n_req) m = mine(a, kd_request(a, next + lane, ROWS, KT, false));
                 const unsigned b = __ballot_sync(0xffffffffu, m);
                 if (b || next >= a.n_req) {
                     next += b ? __ffs(b) - 1 : 0;
@@ -182,7 +191,7 @@ struct KPWalk {
         int rest = (cur - base) - s.h * per_head, gi = 0, lo = 0, t = 0;
         for (int g0 = 0; g0 < q.groups; g0 += 32) {
             t = 0;
-            if (g0 + lane < q.groups) kp_group(a, q, ROWS, g0 + lane, &lo, &t);
+            if (g0 + lane < q.groups) kp_group<KT>(a, q, ROWS, g0 + lane, &lo, &t);
             int v = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -210,8 +219,8 @@ struct KPWalk {
         for (int x = 0; x < 2; ++x) {
             const int r_lo = s.row0 + (ROWS == 256 ? 128 * x : 0), r_hi = min(r_lo + 128, s.row0 + s.nrows) - 1;
             const int first = q.kv - q.n + r_lo / a.G, last = q.kv - q.n + r_hi / a.G;
-            s.lo[x] = a.window > 0 ? max(0, first - a.window + 1) / KP_KT : 0;
-            s.hi[x] = r_hi < r_lo || last < 0 ? -1 : last / KP_KT;
+            s.lo[x] = a.window > 0 ? max(0, first - a.window + 1) / KT : 0;
+            s.hi[x] = r_hi < r_lo || last < 0 ? -1 : last / KT;
         }
         return s;
     }
@@ -319,7 +328,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     kv8_prefill_kernel(const KAttnArgs a, const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v) {
     using S = KPShape<HD, SPLIT>;
-    constexpr int ROWS = S::ROWS, LINE = HD == 64 ? 64 : 128;
+    constexpr int ROWS = S::ROWS, KT = S::KT, HDO = S::HDO, LINE = HD == 64 ? 64 : 128;
+    constexpr bool HALVES = S::HALVES, SHARED = SPLIT || HALVES;  // SHARED: both streams have the same rows
     extern __shared__ __align__(128) uint8_t smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -361,14 +371,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     pdl_wait();
     pdl_launch_dependents();
     // ---- where this CTA's run begins: prefix sums over the requests, in the space of the operands
-    KPWalk<ROWS> walk;
+    KPWalk<ROWS, KT> walk;
     walk.lane = lane;
     {
         int* s_cnt = reinterpret_cast<int*>(smem);  // [n_req] tiles of each
         long long* s_w = reinterpret_cast<long long*>(smem + 4 * FENCE_PAGED_MAX_REQ);
         for (int r0 = warp * 32; r0 < a.n_req; r0 += KP_THREADS) {
             KReq q{};
-            if (r0 + lane < a.n_req) q = kd_request(a, r0 + lane, ROWS, KP_KT, blockIdx.x == 0);
+            if (r0 + lane < a.n_req) q = kd_request(a, r0 + lane, ROWS, KT, blockIdx.x == 0);
             unsigned todo = __ballot_sync(0xffffffffu, walk.mine(a, q));
             int own = 0;
             while (todo) {  // few: requests with many rows
@@ -437,13 +447,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         // ---------------------------------------------------------------- codes -> fp16 operands
         // 8 keys x 64 channels a warp and step; rows r and r ^ 5 side by side: neither the loads nor the stores of a
         // quarter-warp meet on a bank (the staged codes are swizzled too)
-        constexpr int HALF = HD / 64, STEPS = KP_KT / 8 * HALF / 4, STEP_ROWS = 4 / HALF * 8;
+        constexpr int HALF = HD / 64, STEPS = KT / 8 * HALF / 4, STEP_ROWS = 32 / HALF;
         const int cw = warp - KP_W_CONV, r8 = (lane >> 3) ^ ((lane >> 2 & 1) * 5);
         // this thread's row in the first step, its place in the operand and in the stage
-        const int row0 = (cw / HALF) * 8 + r8, half = cw % HALF, c16 = half * 4 + (lane & 3);
-        const uint32_t dst0 = (uint32_t)(half * (KP_KT * 128) + row0 * 128 + (((2 * (lane & 3)) ^ r8) << 4));
+        const int row0 = (cw / HALF) * 8 + r8, half = cw % HALF, c16 = (half & 1) * 4 + (lane & 3);
+        const uint32_t dst0 = (uint32_t)(half * (KT * 128) + row0 * 128 + (((2 * (lane & 3)) ^ r8) << 4));
         const uint32_t raw0 = sbase + S::O_RAW + (HD == 64 ? (uint32_t)(row0 * 64 + ((c16 ^ ((row0 >> 1) & 3)) << 4))
-                                                           : (uint32_t)(row0 * 128 + ((c16 ^ r8) << 4)));
+                                                           : (uint32_t)((half >> 1) * (KT * 128) + row0 * 128 + ((c16 ^ r8) << 4)));
         uint32_t it = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
@@ -453,8 +463,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const int t1 = min(g.tile0 + g.cnt - 1, max(g.hi[0], g.hi[1]));
             for (int kt = t0; kt <= t1; ++kt, ++it) {
                 const uint32_t b = it & 1u;
-                const int lo = any_lo - kt * KP_KT - row0, hi = g.q.kv - kt * KP_KT - row0;
-                const bool edge = hi + row0 < KP_KT || lo + row0 > 0;  // keys there may hold anything: they count as zero
+                const int lo = any_lo - kt * KT - row0, hi = g.q.kv - kt * KT - row0;
+                const bool edge = hi + row0 < KT || lo + row0 > 0;  // keys there may hold anything: they count as zero
 #pragma unroll 1
                 for (int v = 0; v < 2; ++v) {
                     wait(&raw_full[v], it);
@@ -494,7 +504,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         }
     } else if (warp == KP_W_LOAD) {
         // ---------------------------------------------------------------- codes into the stages
-        const int box = min(a.c.page_tokens, 64), boxes = KP_KT / box;
+        const int box = min(a.c.page_tokens, 64), boxes = KT / box;
         uint32_t it = 0, segs = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
@@ -504,7 +514,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 if (!kp_active<SPLIT>(g, 0, kt) && !kp_active<SPLIT>(g, 1, kt)) continue;
                 const uint32_t slot = it % KP_SLOTS;
                 wait(&prep_full[slot], it / KP_SLOTS);
-                const bool load = lane < boxes && kt * KP_KT + lane * box < g.q.kv;
+                const bool load = lane < boxes && kt * KT + lane * box < g.q.kv;
                 const int y = load ? s_row[slot * 8 + lane * (box / 16)] : 0, n = __popc(__ballot_sync(0xffffffffu, load));
                 if (lane == 0) mbar_arrive(&prep_empty[slot]);
 #pragma unroll 1
@@ -514,7 +524,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     if (!ok) break;
                     if (lane == 0) mbar_arrive_expect_tx(&raw_full[v], (uint32_t)(n * box * HD));
                     __syncwarp();
-                    if (load) kd_tma(sbase + S::O_RAW + v * S::RAW + lane * box * LINE, v ? &tm_v : &tm_k, 0, y, &raw_full[v]);
+                    if (load) {
+#pragma unroll
+                        for (int x = 0; x < (HALVES ? 2 : 1); ++x)
+                            kd_tma(sbase + S::O_RAW + v * S::RAW + x * KT * 128 + lane * box * LINE, v ? &tm_v : &tm_k, x * 128, y,
+                                   &raw_full[v]);
+                    }
                 }
                 ++it;
                 if (q_due && ok) {  // the unit's q rows, behind its first tile; once the last unit's scores are done
@@ -525,8 +540,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         const int per_head = a.n_tokens * a.G, y = g.h * per_head + g.q.start * a.G + g.row0;
 #pragma unroll
                         for (int s = 0; s < 2; ++s) {
+                            if (HALVES && s == 1) continue;
                             if (!SPLIT && max(g.lo[s], g.tile0) > min(g.hi[s], g.tile0 + g.cnt - 1)) continue;  // no rows here
-                            uint64_t* full = &q_full[SPLIT ? 0 : s];
+                            uint64_t* full = &q_full[SHARED ? 0 : s];
                             if (!SPLIT || s == 0) mbar_arrive_expect_tx(full, (SPLIT ? 2 : 1) * S::Q_TILE);
 #pragma unroll
                             for (int x = 0; x < HD / 64; ++x)
@@ -547,11 +563,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const KPSeg g = walk.seek(a, cur, end);
             const int* table = a.block_table + (size_t)walk.r * a.max_pages;
             for (int j = 0; j < g.cnt; ++j) {
-                const int kt = g.tile0 + j, key = kt * KP_KT + lane * 16;
+                const int kt = g.tile0 + j, key = kt * KT + lane * 16;
                 if (!kp_active<SPLIT>(g, 0, kt) && !kp_active<SPLIT>(g, 1, kt)) continue;
                 int unit = 0;
                 float ks = 0.f, vs = 0.f;
-                if (lane < 8 && key < g.q.kv) {
+                if (lane < KT / 16 && key < g.q.kv) {
                     int p = table[key >> a.shift];
                     if (p < 0 || p >= a.c.n_pages) {
                         set_device_error(KV8_BAD);
@@ -564,7 +580,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 const uint32_t slot = it % KP_SLOTS;
                 if (it >= KP_SLOTS) wait(&prep_empty[slot], it / KP_SLOTS - 1);
                 __syncwarp();
-                if (lane < 8) {
+                if (lane < KT / 16) {
                     float lv = -INFINITY, rv = 1.f;
                     if (vs > 0.f && vs < INFINITY) {
                         lv = log2f(vs);
@@ -587,7 +603,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     } else if (warp == KP_W_MMA) {
         // ---------------------------------------------------------------- products
         // one copy of the code for both streams: it runs four times a tile and should find itself in the instruction cache
-        constexpr uint32_t id_s = tg_idesc(128, KP_KT), id_o = tg_idesc(128, HD) | (1u << 16);  // V: MN-major
+        constexpr uint32_t id_s = tg_idesc(128, KT), id_o = tg_idesc(128, HDO) | (1u << 16);  // V: MN-major
         const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
         uint32_t it = 0, nq = 0, np = 0, segs = 0;  // nq, np: 16 bits per stream, of which the lowest counts
         for (int cur = begin; cur < end;) {
@@ -618,12 +634,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         }
                         kp_fence_after();
                         const uint32_t d = __shfl_sync(0xffffffffu, tm + 256 + 128 * s, 0), ta = __shfl_sync(0xffffffffu, tm + 128 * s, 0);
-                        const uint64_t db = kp_desc_mn(__shfl_sync(0xffffffffu, sbase + S::O_V + pb * S::OP, 0), KP_KT * 128);
+                        const uint64_t db = kp_desc_mn(__shfl_sync(0xffffffffu, sbase + S::O_V + pb * S::OP + (HALVES ? s * 2 * KT * 128 : 0), 0), KT * 128);
                         if (kp_elect() && ok) {
 #pragma unroll
                             for (int x = 0; x < (SPLIT ? 2 : 1); ++x)
 #pragma unroll
-                                for (int k = 0; k < KP_KT / 16; ++k)  // 16 keys: 2048 bytes further
+                                for (int k = 0; k < KT / 16; ++k)  // 16 keys: 2048 bytes further
                                     kp_mma_ts(d, ta + (k >> 1) * 32 + x * 16 + (k & 1) * 8, db + k * 128, id_o, x > 0 || k > 0 ? 1u : add);
                             if (((left >> (8 * pb)) & 255u) == 0) kp_commit(&v_empty[pb]);
                         }
@@ -631,7 +647,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         else pend0 = -1;
                     }
                     if (act) {  // S_s = Q_s . K^T
-                        const int qi = SPLIT ? 0 : s;
+                        const int qi = SHARED ? 0 : s;
                         if (!((have >> qi) & 1u)) {
                             have |= 1u << qi;
                             wait(&q_full[qi], nq >> (16 * qi));
@@ -649,7 +665,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
                                 for (int k = 0; k < HD / 16; ++k)
                                     kp_mma_ss(d, da + (x * S::Q_TILE + (k >> 2) * 128 * 128 + (k & 3) * 32) / 16,
-                                              db + ((k >> 2) * KP_KT * 128 + (k & 3) * 32) / 16, id_s, (SPLIT && x == 0) || k > 0);
+                                              db + ((k >> 2) * KT * 128 + (k & 3) * 32) / 16, id_s, (SPLIT && x == 0) || k > 0);
                             kp_commit(&s_full[s]);
                         }
                         if (s) pend1 = (int)it;
@@ -689,15 +705,16 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         }
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
-            const int i_row = (SPLIT ? 0 : 128 * s) + row;  // in the group
+            const int i_row = (SHARED ? 0 : 128 * s) + row;  // in the group
             const bool valid = i_row < g.nrows;
             const int tok_i = (g.row0 + (valid ? i_row : 0)) / a.G;
             const int head = g.h * a.G + (g.row0 + (valid ? i_row : 0)) % a.G;
             const long long tok = g.q.start + tok_i;
+            const int ch0 = HALVES ? s * HDO : 0;  // this stream's channels
             const int lim = valid ? g.q.kv - g.q.n + tok_i : -1;
             const int lim_lo = a.window > 0 ? lim - a.window + 1 : 0;
             // tiles that all of this stream's rows see whole need no mask
-            const int r_lo = g.row0 + (SPLIT ? 0 : 128 * s), r_hi = min(r_lo + 128, g.row0 + g.nrows) - 1;
+            const int r_lo = g.row0 + (SHARED ? 0 : 128 * s), r_hi = min(r_lo + 128, g.row0 + g.nrows) - 1;
             const int lim_first = g.q.kv - g.q.n + r_lo / a.G, lim_last = g.q.kv - g.q.n + r_hi / a.G;
             const float qs = valid ? a.q_scale[(long long)g.h * a.n_tokens * a.G + tok * a.G + (g.row0 + i_row) % a.G] : 1.f;
             float m = -INFINITY, l = 0.f, lvref = -INFINITY, vref = 0.f;
@@ -710,7 +727,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 const float f = drained ? kd_exp2(m_rec - (m == -INFINITY ? 0.f : m)) : 0.f;
                 float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
+                for (int c = 0; c < HDO; c += 16) {
                     uint32_t r[16];
                     if (have_o) {
                         KP_LD16(r, t_o + c);
@@ -735,7 +752,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 m_rec = m;
             };
             for (int j = 0; j < g.cnt; ++j) {
-                const int kt = g.tile0 + j, key0 = kt * KP_KT;
+                const int kt = g.tile0 + j, key0 = kt * KT;
                 const bool act = kp_active<SPLIT>(g, s, kt);
                 if (!act && !kp_active<SPLIT>(g, 1 - s, kt)) continue;
                 const uint32_t slot = it % KP_SLOTS, use = it / KP_SLOTS;
@@ -758,11 +775,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 if (SPLIT) ++since;
                 const float* pr = s_prep + slot * 24;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
                 // Loops of 32 columns, not unrolled: the roles' code has to share the instruction cache.
-                const bool edge = key0 + KP_KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
+                const bool edge = key0 + KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
                 uint32_t bad = 0;  // of an edge tile: blocks of 16 keys with a scale that is no number, of which this row sees some
                 if (edge) {        // -infinity in the columns that this row does not see
 #pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < KT / 32; ++c) {
                         uint32_t x[32];
                         KP_LD32(x, t_s + 32 * c);
                         kp_wait_ld();
@@ -788,7 +805,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 constexpr int CH = 32, NB = CH / 16;
                 float mt = -INFINITY, lvmax = -INFINITY;
 #pragma unroll 1
-                for (int c = 0; c < KP_KT; c += CH) {
+                for (int c = 0; c < KT; c += CH) {
                     uint32_t x[CH];
 #pragma unroll
                     for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
@@ -820,7 +837,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     m = mn;
                     if (have_o) {  // the products of the tiles before have ended: S came after them
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 16) {
+                        for (int c = 0; c < HDO; c += 16) {
                             uint32_t r[16];
                             KP_LD16(r, t_o + c);
                             kp_wait_ld();
@@ -834,7 +851,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 const float mm = m == -INFINITY ? 0.f : m, lv0 = lvref == -INFINITY ? 0.f : lvref;
                 // ---- weights, in place of the scores
 #pragma unroll 1
-                for (int c = 0; c < KP_KT; c += CH) {
+                for (int c = 0; c < KT; c += CH) {
                     uint32_t x[CH];
 #pragma unroll
                     for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
@@ -898,7 +915,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 const float mul = direct ? (l == 0.f ? 0.f : vref / l) : vref;
                 float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
 #pragma unroll 1
-                for (int c = 0; c < HD; c += 16) {
+                for (int c = 0; c < HDO; c += 16) {
                     uint32_t r[16];
                     float x[16];
                     if (have_o) {
@@ -908,7 +925,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) x[e] = have_o && mul != 0.f ? __uint_as_float(r[e]) * mul : 0.f;
                     if (direct) {
-                        const long long at = tok * a.out_stride + (long long)head * HD + c;
+                        const long long at = tok * a.out_stride + (long long)head * HD + ch0 + c;
                         if (valid) {
                             kv8_st8(a.out, at, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x));
                             kv8_st8(a.out, at + 8, a.type, a.out_wide, *reinterpret_cast<const float(*)[8]>(x + 8));
@@ -921,7 +938,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 }
             }
             if (direct) {
-                if (valid && a.lse) a.lse[tok * a.n_q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
+                if (valid && a.lse && (!HALVES || s == 0)) a.lse[tok * a.n_q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
             } else {
                 __stcg(reinterpret_cast<float2*>(record()) + row, make_float2(m, l));
                 __threadfence();
@@ -937,7 +954,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 if (s_misc[4]) {
                     // join the parts in the order of the keys; SPLIT: both streams' parts of the same rows, half the channels each
                     constexpr int STREAMS = SPLIT ? 2 : 1;
-                    const int c0 = SPLIT ? s * (HD / 2) : 0, c1 = SPLIT ? c0 + HD / 2 : HD;
+                    const int c0 = SPLIT ? s * (HD / 2) : 0, c1 = SPLIT ? c0 + HD / 2 : HDO;
                     float M = -INFINITY, L = 0.f;
 #pragma unroll 1
                     for (int k = c_first; k <= c_last; ++k)
@@ -976,11 +993,11 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                                 float x[8];
 #pragma unroll
                                 for (int y = 0; y < 8; ++y) x[y] = acc[e + y] * inv;
-                                kv8_st8(a.out, tok * a.out_stride + (long long)head * HD + c + e, a.type, a.out_wide, x);
+                                kv8_st8(a.out, tok * a.out_stride + (long long)head * HD + ch0 + c + e, a.type, a.out_wide, x);
                             }
                         }
                     }
-                    if (valid && a.lse && (!SPLIT || s == 0))
+                    if (valid && a.lse && (!SHARED || s == 0))
                         a.lse[tok * a.n_q_heads + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.693147180559945f;
                 }
             }
