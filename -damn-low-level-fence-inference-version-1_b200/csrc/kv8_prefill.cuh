@@ -32,6 +32,7 @@ namespace fence {
 constexpr int KP_SMS = 148;
 constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_W_LOAD = 14, KP_THREADS = 480;
 constexpr int KP_MIN_TILES = 2, KP_SLOTS = 4;
+constexpr int KP_UNIT = 4;  // a unit's start and end cost about as much as four tiles: counted so when the runs are cut
 // SPLIT: the matrix unit's additions cut the sum's last bit off, half of it on average and always towards zero: 128 of
 // them (8 tiles) cost 2e-6. So after every 4 tiles of a stream the sums are added, rounded, to the stream's record.
 constexpr int KP_DRAIN = 4;
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(32 * KQ_WARPS) kv8_q_rows_kernel(const KAttnAr
 struct KPSeg {
     KReq q;
     int h, row0, nrows, tile0, cnt, first, tiles;  // this CTA's tiles of the unit, its place in the unit, the unit's tiles
+    int unit0, next;                               // where the unit's place in the list begins, where this CTA's next one is
     int lo[2], hi[2];                              // the tiles that rows of each stream see
 };
 
@@ -154,7 +156,10 @@ struct KPWalk {
         int sum = 0;
         for (int g0 = 0; g0 < x.groups; g0 += 32) {
             int lo, t = 0;
-            if (g0 + lane < x.groups) kp_group<KT>(a, x, ROWS, g0 + lane, &lo, &t);
+            if (g0 + lane < x.groups) {
+                kp_group<KT>(a, x, ROWS, g0 + lane, &lo, &t);
+                t += KP_UNIT;
+            }
             sum += __reduce_add_sync(0xffffffffu, (unsigned)t);
         }
         return sum;
@@ -191,7 +196,10 @@ struct KPWalk {
         int rest = (cur - base) - s.h * per_head, gi = 0, lo = 0, t = 0;
         for (int g0 = 0; g0 < q.groups; g0 += 32) {
             t = 0;
-            if (g0 + lane < q.groups) kp_group<KT>(a, q, ROWS, g0 + lane, &lo, &t);
+            if (g0 + lane < q.groups) {
+                kp_group<KT>(a, q, ROWS, g0 + lane, &lo, &t);
+                t += KP_UNIT;
+            }
             int v = t;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -211,10 +219,12 @@ struct KPWalk {
         }
         s.row0 = gi * ROWS;
         s.nrows = min(ROWS, q.n * a.G - s.row0);
-        s.first = rest;
-        s.tiles = t;
-        s.tile0 = lo + rest;
-        s.cnt = min(t - rest, end - cur);
+        s.unit0 = cur - rest;
+        s.tiles = t - KP_UNIT;
+        s.first = max(0, rest - KP_UNIT);
+        s.tile0 = lo + s.first;
+        s.cnt = min(s.tiles, end - s.unit0 - KP_UNIT) - s.first;  // none: the run ends in this unit's start, its tiles are the next CTA's
+        s.next = s.cnt > 0 ? s.unit0 + KP_UNIT + s.first + s.cnt : INT_MAX;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const int r_lo = s.row0 + (ROWS == 256 ? 128 * x : 0), r_hi = min(r_lo + 128, s.row0 + s.nrows) - 1;
@@ -416,7 +426,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             if (tid == 0) set_device_error(KV8_BAD);
             all = 0;  // no such list fits a pool
         }
-        const int per = max(KP_MIN_TILES, (int)((all + gridDim.x - 1) / gridDim.x));
+        const int per = max(KP_MIN_TILES + KP_UNIT, (int)((all + gridDim.x - 1) / gridDim.x));
         const long long begin = (long long)blockIdx.x * per;
         if (tid == 0) s_misc[1] = (int)all;
         long long at = v - sum;
@@ -430,7 +440,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         __syncthreads();
     }
     const int total = s_misc[1];
-    const int per = max(KP_MIN_TILES, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    const int per = max(KP_MIN_TILES + KP_UNIT, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     const int begin = (int)min((long long)total, (long long)blockIdx.x * per), end = min(total, begin + min(per, total - begin));
     if (begin < end) walk.enter(a, s_misc[2], s_misc[3]);
     kp_fence_before();
@@ -457,6 +467,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         uint32_t it = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
+            if (g.cnt <= 0) break;
             const int any_lo = a.window > 0 ? max(0, g.q.kv - g.q.n + g.row0 / a.G - a.window + 1) : 0;
             // the tiles that some row sees follow one another
             const int t0 = max(g.tile0, min(g.hi[0] < 0 ? INT_MAX : g.lo[0], g.hi[1] < 0 ? INT_MAX : g.lo[1]));
@@ -500,7 +511,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     }
                 }
             }
-            cur += g.cnt;
+            cur = g.next;
         }
     } else if (warp == KP_W_LOAD) {
         // ---------------------------------------------------------------- codes into the stages
@@ -508,6 +519,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         uint32_t it = 0, segs = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
+            if (g.cnt <= 0) break;
             bool q_due = true;
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j;
@@ -554,13 +566,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 }
             }
             ++segs;
-            cur += g.cnt;
+            cur = g.next;
         }
     } else if (warp == KP_W_PREP) {
         // ---------------------------------------------------------------- pages and scales of 8 x 16 keys, some tiles ahead
         uint32_t it = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
+            if (g.cnt <= 0) break;
             const int* table = a.block_table + (size_t)walk.r * a.max_pages;
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j, key = kt * KT + lane * 16;
@@ -598,7 +611,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 if (lane == 0) mbar_arrive(&prep_full[slot]);
                 ++it;
             }
-            cur += g.cnt;
+            cur = g.next;
         }
     } else if (warp == KP_W_MMA) {
         // ---------------------------------------------------------------- products
@@ -608,6 +621,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         uint32_t it = 0, nq = 0, np = 0, segs = 0;  // nq, np: 16 bits per stream, of which the lowest counts
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
+            if (g.cnt <= 0) break;
             int pend0 = -1, pend1 = -1;      // the tile (count) whose weights a stream is making
             uint32_t have = 0, left = 0, made[2] = {0, 0};  // have: q (bits 0, 1) and o (2, 3) of the streams; left: streams that still need V, 8 bits per buffer
             const int last = g.tile0 + g.cnt;
@@ -686,7 +700,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             ++segs;
             if (kp_elect() && ok) kp_commit(o_full);
             __syncwarp();
-            cur += g.cnt;
+            cur = g.next;
         }
     } else if (warp < KP_W_CONV) {
         // ---------------------------------------------------------------- softmax, a thread per row
@@ -705,6 +719,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
         }
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
+            if (g.cnt <= 0) break;
             const int i_row = (SHARED ? 0 : 128 * s) + row;  // in the group
             const bool valid = i_row < g.nrows;
             const int tok_i = (g.row0 + (valid ? i_row : 0)) / a.G;
@@ -907,8 +922,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             __syncwarp();
             kp_fence_after();
             const bool whole = g.cnt == g.tiles, direct = whole && !SPLIT;
-            const int unit0 = cur - g.first;
-            const int c_first = unit0 / per, c_last = (unit0 + g.tiles - 1) / per;
+            const int c_first = (g.unit0 + KP_UNIT) / per, c_last = (g.unit0 + KP_UNIT + g.tiles - 1) / per;
             if (SPLIT) {
                 drain();
             } else {  // out, or to the record
@@ -1004,7 +1018,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             kp_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(seg_done);
-            cur += g.cnt;
+            cur = g.next;
         }
     }
     kp_fence_before();
