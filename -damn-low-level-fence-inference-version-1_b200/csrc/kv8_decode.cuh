@@ -5,7 +5,7 @@
 // Bound: HBM, two bytes per key, head and channel; the kernel has to keep the codes coming and turn them
 // into matrix operands fast enough.
 //
-//  * Work is the list of 64-key tiles of every (request, KV head, group of 8 NT query rows), cut into
+//  * Work is the list of 32-key tiles of every (request, KV head, group of 8 NT query rows), cut into
 //    runs of equal cost, one per CTA, whatever the lengths are: a CTA's run may begin and end inside a unit. Such a
 //    unit's partial results go to the workspace and the last of its CTAs to arrive joins them in the
 //    order of the keys, so the result does not depend on timing.
@@ -49,16 +49,17 @@ struct KAttnArgs {
     float* part;       // [CTAs][2][rows * (head_dim + 2)]
 };
 
-constexpr int KD_TILE = 64, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
-constexpr int KD_MIN_TILES = 2;  // tiles per CTA below which more CTAs only add joins
-constexpr int KD_UNIT = 4;       // a unit's start and end cost about as much as four tiles: counted so when the runs are cut
+constexpr int KD_TILE = 32, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
+constexpr int KD_MIN_TILES = 4;  // tiles per CTA below which more CTAs only add joins
+constexpr int KD_UNIT = 8;       // a unit's start and end cost about as much as eight tiles: counted so when the runs are cut
 constexpr float KD_LAZY = 8.f;   // the running maximum may lag by 2^8: fp16 weights stay below 2^16
 
 template <int HD, bool SPLIT, int NT>
 struct KDShape {
     // CTAs per SM, by the registers that the sums take
     static constexpr int CTAS = HD == 256 ? (NT == 2 ? 1 : 2) : (HD == 128 && NT == 2 ? 2 : 3);
-    static constexpr int STAGES = HD == 64 ? 8 : HD == 128 ? (CTAS == 3 ? 4 : 6) : NT == 2 ? 5 : 3;
+    // twice as many stages as warps: with one each, every tile's load began when the tile before it was done with
+    static constexpr int STAGES = HD == 64 ? 12 : HD == 128 ? (CTAS == 3 ? 8 : 12) : NT == 2 ? 10 : 6;
     static constexpr int KV_BYTES = KD_TILE * HD;
     static constexpr int STAGE = 2 * KV_BYTES;
     static constexpr int ROWS = 8 * NT;
@@ -366,7 +367,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                     sk[y] = s_scale[s * 8 + y * 16 / box];
                     sv[y] = s_scale[s * 8 + 4 + y * 16 / box];
                 }
-                // ---- scores of 64 keys: four products side by side
+                // ---- scores of 32 keys: two products side by side
                 float acc[MK][NT][4], low[SPLIT ? MK : 1][NT][4];
 #pragma unroll
                 for (int y = 0; y < MK; ++y)
