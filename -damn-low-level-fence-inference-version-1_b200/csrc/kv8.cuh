@@ -50,8 +50,10 @@ __device__ __forceinline__ uint32_t kd_half2(uint32_t w, bool high) {
         const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
         return *reinterpret_cast<const uint32_t*>(&h);
     }
-    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(high ? w >> 16 : w & 0xffffu), __NV_E4M3);
-    return (uint32_t)r.x | ((uint32_t)r.y << 16);
+    uint32_t h;
+    if (high) asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, u;\n\t}" : "=r"(h) : "r"(w));
+    else asm("{\n\t.reg .b16 l, u;\n\tmov.b32 {l, u}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(h) : "r"(w));
+    return h;
 }
 template <int FMT>
 __device__ __forceinline__ uint32_t kd_bias(uint32_t w) { return FMT == KV8_INT8 ? w ^ 0x80808080u : w; }

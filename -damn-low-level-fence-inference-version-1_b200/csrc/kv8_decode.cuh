@@ -364,8 +364,8 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                 float sk[MK], sv[MK];
 #pragma unroll
                 for (int y = 0; y < MK; ++y) {
-                    sk[y] = s_scale[s * 8 + y * 16 / box];
-                    sv[y] = s_scale[s * 8 + 4 + y * 16 / box];
+                    sk[y] = s_scale[s * 8 + (box == 16 ? y : 0)];  // a box of 32 keys holds the tile
+                    sv[y] = s_scale[s * 8 + 4 + (box == 16 ? y : 0)];
                 }
                 // ---- scores of 32 keys: two products side by side
                 float acc[MK][NT][4], low[SPLIT ? MK : 1][NT][4];
@@ -477,21 +477,30 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                         }
                 }
                 // ---- the weights as B fragments, with the V scale over its reference
+                float mm[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) mm[nt][e] = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
                 uint32_t b0[MK][NT], b1[MK][NT], c0[SPLIT ? MK : 1][NT], c1[SPLIT ? MK : 1][NT];
 #pragma unroll
                 for (int y = 0; y < MK; ++y) {
                     // a NaN or infinite scale gives NaN to whoever sees the key
                     const float fv = !(sv[y] < INFINITY) ? __uint_as_float(0x7fffffffu) : vref > 0.f ? sv[y] * vinv : 1.f;
+                    const bool apart = masked && !(fv < INFINITY);  // to nobody else
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float p[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float mm = m[nt][e & 1] == -INFINITY ? 0.f : m[nt][e & 1];
-                            const float x = kd_exp2(acc[y][nt][e] - mm);
+                            const float x = kd_exp2(acc[y][nt][e] - mm[nt][e & 1]);
                             l[nt][e & 1] += x;
                             p[e] = x * fv;
-                            if (masked && acc[y][nt][e] == -INFINITY) p[e] = 0.f;
+                        }
+                        if (apart) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if (acc[y][nt][e] == -INFINITY) p[e] = 0.f;
                         }
                         const uint32_t h0 = kd_pack(p[0], p[1]), h1 = kd_pack(p[2], p[3]);
                         b0[y][nt] = kd_transpose(h0);
