@@ -1,9 +1,10 @@
-// kv8_decode.cuh — attention of a few query rows per request over the paged 8-bit cache (decode, drafts).
+// kv8_decode.cuh — attention of up to 48 query rows per request and KV head over the paged 8-bit cache (decode, drafts).
 //
 //   s[j][h] = (K code row j . q row h) * k_scale[page] * scale,  p = softmax(s),  out = p . (V code rows * v_scale[page])
 //
 // Bound: HBM, two bytes per key, head and channel; the kernel has to keep the codes coming and turn them
-// into matrix operands fast enough.
+// into matrix operands fast enough. 3 requests of 90k to 131k keys, 8 heads of 128, e4m3: 639 MB in 117 us (84 % of the
+// measured copy bandwidth); 64 requests of 60 to 8000 keys: 199 MB in 50 us, a third of it starts and ends of units.
 //
 //  * Work is the list of 32-key tiles of every (request, KV head, group of 8 NT query rows), cut into
 //    runs of equal cost, one per CTA, whatever the lengths are: a CTA's run may begin and end inside a unit. Such a

@@ -6,7 +6,8 @@
 //   page j that the call hands out = stack[avail - 1 - j], stack = free pages, then the ended requests' pages
 //   token t belongs to the last request whose start is <= t; its page is its table's entry, or if the
 //   call has just handed it out, page N_r + (pos / P - held) of the call.
-// What bounds it is latency: the launch, the lengths' load, the scans, one dependent load of a page id.
+// What bounds it is latency: the launch, the lengths' load, the scans, one dependent load of a page id
+// (6.5 us alone for 48 requests, 13.5 us for 2000 requests with 46 thousand tokens, cold caches).
 // So every CTA repeats the scans for itself in shared memory (at most 4096 requests: 16 KB of lengths
 // from L2) and then writes its share of the outputs; nothing waits on another CTA, and no CTA reads what
 // another one writes: table entries below `held`, free pages below n_free and the ended requests' rows
@@ -121,7 +122,6 @@ __global__ void paged_plan_kernel(const PlanArgs p) {
         e_new += nw;
         e_need += need;
         e_back += back;
-        // -1: not placed or ended, so that the next step's ctx can be told from kv
         if (blockIdx.x == 0) {
             const int raw = b.new_len[r];
             b.ctx_out[r] = raw < 0 ? 0 : placed ? kv : ctx;
