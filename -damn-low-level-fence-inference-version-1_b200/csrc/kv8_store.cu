@@ -90,63 +90,60 @@ __global__ void __launch_bounds__(512) kv8_store_kernel(const StoreArgs a) {
 struct LoadArgs {
     fence_kv8_cache c;
     const int* slot;
-    int n, shift;
+    int n, shift, rows;  // rows: per block
     void* x[2];
     long long stride[2];
     int type, wide[2];
 };
 
-// A thread takes KV8_LD_ITEMS times 16 codes, all loads in flight together. Bound: HBM (one byte in, one element out).
-constexpr int KV8_LD_ITEMS = 2;
+// A block takes whole rows, about 256 x KV8_LD_ITEMS pieces of 8 codes; a thread's loads are in flight together and a warp's
+// stores fill whole lines. Bound: HBM (one byte in, one element out).
+constexpr int KV8_LD_ITEMS = 4;
 template <int FMT>
 __global__ void __launch_bounds__(256) kv8_load_kernel(const LoadArgs a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int hd = a.c.head_dim, cpr = hd / 16, row = a.c.n_kv_heads * cpr, kv = blockIdx.y, shift = 31 - __clz(cpr);
+    const int hd = a.c.head_dim, cpr = hd / 8, row = a.c.n_kv_heads * cpr, kv = blockIdx.y, shift = 31 - __clz(cpr);
     if (!a.x[kv]) return;
     const uint8_t* codes = static_cast<const uint8_t*>(kv ? a.c.v : a.c.k);
     const float* scale = kv ? a.c.v_scale : a.c.k_scale;
-    // a block's items are consecutive: 32-bit division within the block
-    const long long first = (long long)blockIdx.x * (256 * KV8_LD_ITEMS);
-    const int t0 = (int)(first / row), c0 = (int)(first - (long long)t0 * row);
-    uint4 w[KV8_LD_ITEMS];
-    float s[KV8_LD_ITEMS];
-    int t[KV8_LD_ITEMS], c[KV8_LD_ITEMS];
+    const int t0 = blockIdx.x * a.rows, n = min(a.rows, a.n - t0) * row;
+    for (int base = (int)threadIdx.x; base < n; base += 256 * KV8_LD_ITEMS) {
+        uint2 w[KV8_LD_ITEMS];
+        float s[KV8_LD_ITEMS];
+        int t[KV8_LD_ITEMS], c[KV8_LD_ITEMS];
 #pragma unroll
-    for (int j = 0; j < KV8_LD_ITEMS; ++j) {
-        const int i = c0 + (int)threadIdx.x + j * 256, q = i / row;
-        t[j] = t0 + q;
-        c[j] = i - q * row;
-        w[j] = make_uint4(0, 0, 0, 0);
-        s[j] = 0.f;
-        if (t[j] < a.n) {
-            const int slot = a.slot[t[j]], page = slot >> a.shift, h = c[j] >> shift;
-            if (slot >= 0 && page < a.c.n_pages) {
-                const long long unit = (long long)page * a.c.n_kv_heads + h;
-                w[j] = *reinterpret_cast<const uint4*>(codes + (unit * a.c.page_tokens + (slot & (a.c.page_tokens - 1))) * hd +
-                                                       (c[j] & (cpr - 1)) * 16);
-                s[j] = scale[unit];
-            } else if (slot != -1) {
-                set_device_error(KV8_BAD);
+        for (int j = 0; j < KV8_LD_ITEMS; ++j) {
+            const int i = base + j * 256, q = i / row;
+            t[j] = q;
+            c[j] = i - q * row;
+            w[j] = make_uint2(0, 0);
+            s[j] = 0.f;
+            if (i < n) {
+                const int slot = a.slot[t0 + q], page = slot >> a.shift, h = c[j] >> shift;
+                if (slot >= 0 && page < a.c.n_pages) {
+                    const long long unit = (long long)page * a.c.n_kv_heads + h;
+                    w[j] = *reinterpret_cast<const uint2*>(codes + (unit * a.c.page_tokens + (slot & (a.c.page_tokens - 1))) * hd +
+                                                           (c[j] & (cpr - 1)) * 8);
+                    s[j] = scale[unit];
+                } else if (slot != -1) {
+                    set_device_error(KV8_BAD);
+                }
             }
         }
-    }
 #pragma unroll
-    for (int j = 0; j < KV8_LD_ITEMS; ++j) {
-        if (t[j] >= a.n) continue;
-        const uint32_t y[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int j = 0; j < KV8_LD_ITEMS; ++j) {
+            if (base + j * 256 >= n) continue;
             float v[8];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const uint32_t b = kd_bias<FMT>(y[2 * h + k]), lo = kd_half2<FMT>(b, false), hi = kd_half2<FMT>(b, true);
+                const uint32_t b = kd_bias<FMT>(k ? w[j].y : w[j].x), lo = kd_half2<FMT>(b, false), hi = kd_half2<FMT>(b, true);
                 v[4 * k] = half_bits_to_float(lo) * s[j];
                 v[4 * k + 1] = half_bits_to_float(lo >> 16) * s[j];
                 v[4 * k + 2] = half_bits_to_float(hi) * s[j];
                 v[4 * k + 3] = half_bits_to_float(hi >> 16) * s[j];
             }
-            kv8_st8(a.x[kv], (long long)t[j] * a.stride[kv] + c[j] * 16 + h * 8, a.type, a.wide[kv], v);
+            kv8_st8(a.x[kv], (long long)(t0 + t[j]) * a.stride[kv] + c[j] * 8, a.type, a.wide[kv], v);
         }
     }
 }
@@ -197,6 +194,7 @@ extern "C" int fence_kv8_load(const fence_kv8_cache* c, const int* slot, int n, 
                               long long v_stride, fence_stream_t stream) {
     using namespace fence;
     if (int e = kv8_check_cache(c, "kv8_load")) return e;
+    if (c->n_kv_heads > 65535) return set_error(FENCE_E_UNSUPPORTED, "kv8_load: %d heads", c->n_kv_heads);
     if (n < 0 || (n > 0 && (!slot || (!k && !v)))) return set_error(FENCE_E_ARG, "kv8_load: bad arguments (n=%d)", n);
     if (!kv8_type_ok(type)) return set_error(FENCE_E_UNSUPPORTED, "kv8_load: element type %d", type);
     if (n == 0) return FENCE_OK;
@@ -206,12 +204,10 @@ extern "C" int fence_kv8_load(const fence_kv8_cache* c, const int* slot, int n, 
     const uintptr_t es = (uintptr_t)kv8_elem_size(type);
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % es)
         return set_error(FENCE_E_ALIGN, "kv8_load: k and v must be aligned to their elements");
-    LoadArgs a{*c, slot, n, ilog2(c->page_tokens), {k, v}, {k_stride, v_stride}, type,
+    const int pieces = 256 * KV8_LD_ITEMS, per_row = (int)(row / 8), rows = per_row < pieces ? pieces / per_row : 1;
+    LoadArgs a{*c, slot, n, ilog2(c->page_tokens), rows, {k, v}, {k_stride, v_stride}, type,
                {kv8_wide(k, k_stride, type), kv8_wide(v, v_stride, type)}};
-    const long long items = (long long)n * c->n_kv_heads * (c->head_dim / 16);
-    const long long blocks = (items + 256 * KV8_LD_ITEMS - 1) / (256 * KV8_LD_ITEMS);
-    if (blocks > INT_MAX) return set_error(FENCE_E_UNSUPPORTED, "kv8_load: %d rows", n);
-    const dim3 grid((unsigned)blocks, 2);
+    const dim3 grid((unsigned)((n + (long long)rows - 1) / rows), 2);
     return cuda_status(kv8_launch(c->format == KV8_INT8 ? kv8_load_kernel<KV8_INT8> : kv8_load_kernel<KV8_E4M3>, grid, 256, 0,
                                   (cudaStream_t)stream, a),
                        "kv8_load");
