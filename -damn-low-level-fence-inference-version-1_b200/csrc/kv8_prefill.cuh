@@ -5,7 +5,7 @@
 //
 // Bound: the matrix unit (4 head_dim operations per visible pair) and, as large here, the exponentials:
 // 128 x 128 of them per tile at 16 a clock take as long as the tile's products. 2048 rows of 32 heads of 128 at 30000
-// keys: 1.27 ms, 820 TFLOP/s (half of the measured matrix rate); what is left is the softmax's chain of latencies per tile.
+// keys: 1.29 ms, 810 TFLOP/s (half of the measured matrix rate); what is left is the softmax's chain of latencies per tile.
 //
 //  * Work is the list of 128-key tiles of every (request, KV head, group of query rows), cut into equal
 //    runs, one per CTA, as in the decode kernel: causal groups of any length fill all SMs alike. Units

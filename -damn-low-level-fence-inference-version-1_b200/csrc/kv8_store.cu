@@ -18,7 +18,7 @@ constexpr int KV8_ST_CHUNKS = 8;  // of 8 elements, at most, per thread: a page 
 // pattern of |x| (so that NaN wins over everything), then the page's scale, the older rows if it grew, and
 // the new rows' codes. Bound: HBM, each element read once and its code written once; all of a thread's
 // loads are in flight together and the rows stay in registers between the two steps (read twice, in
-// loops, 8000 rows of 8 x 128 bf16 took 23 us against 7.6 us of traffic). Threads: the page's elements / 64, 128 to 512.
+// loops, 8000 rows of 8 x 128 bf16 took 23 us; so 12.4, against 7.6 us of traffic). Threads: the page's elements / 64, 128 to 512.
 template <int FMT, int TYPE, bool WIDE>
 __global__ void __launch_bounds__(512) kv8_store_kernel(const StoreArgs a) {
     pdl_launch_dependents();
@@ -97,7 +97,8 @@ struct LoadArgs {
 };
 
 // A block takes whole rows, about 256 x KV8_LD_ITEMS pieces of 8 codes; a thread's loads are in flight together and a warp's
-// stores fill whole lines. Bound: HBM (one byte in, one element out).
+// stores fill whole lines. Bound: HBM (one byte in, one element out): 8000 rows of 8 x 128 to bf16 16.1 us against 7.6 us of
+// traffic, the rest the chain slot, page, codes.
 constexpr int KV8_LD_ITEMS = 4;
 template <int FMT>
 __global__ void __launch_bounds__(256) kv8_load_kernel(const LoadArgs a) {
