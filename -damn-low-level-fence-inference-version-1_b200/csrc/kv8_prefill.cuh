@@ -517,7 +517,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
     } else if (warp == KP_W_LOAD) {
         // ---------------------------------------------------------------- codes into the stages
         const int box = min(a.c.page_tokens, 64), boxes = KT / box;
-        uint32_t it = 0, segs = 0;
+        // fetched: units whose q rows were fetched. Units with no tile that a row sees (a prompt that was not placed) have none, and
+        // no phase of q_empty: both sides count the same units, or a wait by parity would pass a unit too early.
+        uint32_t it = 0, fetched = 0;
         for (int cur = begin; cur < end;) {
             const KPSeg g = walk.seek(a, cur, end);
             if (g.cnt <= 0) break;
@@ -547,7 +549,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 ++it;
                 if (q_due && ok) {  // the unit's q rows, behind its first tile; once the last unit's scores are done
                     q_due = false;
-                    if (segs > 0) wait(q_empty, segs - 1);
+                    if (fetched > 0) wait(q_empty, fetched - 1);
+                    ++fetched;
                     ok = __all_sync(0xffffffffu, ok);
                     if (ok && lane == 0) {
                         const int per_head = a.n_tokens * a.G, y = g.h * per_head + g.q.start * a.G + g.row0;
@@ -566,7 +569,6 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     __syncwarp();
                 }
             }
-            ++segs;
             cur = g.next;
         }
     } else if (warp == KP_W_PREP) {
@@ -694,7 +696,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     ++it;
                 }
             }
-            if (kp_elect() && ok) kp_commit(q_empty);
+            if ((have & 3u) && kp_elect() && ok) kp_commit(q_empty);  // only where scores were made: the loader's count
             __syncwarp();
             // a stream without tiles here may still be at the last unit's end: o_full must not run two ahead of it
             if (segs > 0) wait(seg_done, segs - 1);

@@ -1,0 +1,46 @@
+"""Batches of the paged 8-bit attention in which requests that see nothing stand between others, against the row-by-row
+definition (tests/kv8_ref.py) within the bounds of tests/test_kv8_gpu.py."""
+import random
+
+import pytest
+
+from test_kv8_gpu import Batch, T, ref  # noqa: F401  (T and ref are fixtures)
+
+pytestmark = pytest.mark.gpu
+
+# 4 query heads per KV head: more than 12 new tokens are more than 48 rows. 30 rows are one group of 120, seen by nobody;
+# with an odd number of KV heads an odd number of such units follow one another.
+KINDS = [(1, 64, 0), (1, 128, 1), (1, 128, 0), (1, 256, 2), (5, 64, 1), (5, 128, 0), (5, 128, 2), (3, 256, 1)]
+
+
+@pytest.mark.parametrize("hkv,hd,type", KINDS)
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_prompts_not_placed_between_prompts(fb, T, ref, hkv, hd, type, fmt):  # noqa: F811
+    """Short prompts, every other one not placed: a CTA's run of tiles crosses several units without tiles."""
+    rng = random.Random(hkv * hd + type)
+    lens = []
+    for _ in range(300 // hkv):
+        n = rng.choice([30, 32, 64])
+        lens.append((rng.randint(n, 400), n))
+        lens.append((0, 30))
+    Batch(fb, T, lens, 4 * hkv, hkv, hd, 64, fmt, type).check(ref)
+
+
+@pytest.mark.parametrize("hkv,hd,type", KINDS)
+def test_long_prompts_with_gaps_of_every_length(fb, T, ref, hkv, hd, type):  # noqa: F811
+    """Units of many tiles with none, one, two or three requests that were not placed between them, decode rows among them."""
+    rng = random.Random(7 * hkv + hd)
+    lens = []
+    for i in range(28 // hkv):
+        lens.append((rng.randint(1500, 4000), rng.choice([60, 130, 256])))
+        lens += [(0, rng.choice([30, 60, 70])) for _ in range(i % 4)] + [(rng.randint(1, 300), 1)]
+    Batch(fb, T, lens, 4 * hkv, hkv, hd, 32, 0, type).check(ref)
+
+
+@pytest.mark.parametrize("hkv,hd,type", KINDS)
+def test_rows_before_the_first_position(fb, T, ref, hkv, hd, type):  # noqa: F811
+    """More rows than positions: the first groups of rows of a request see nothing, the later ones do."""
+    lens = []
+    for i in range(120 // hkv):
+        lens += [(50 + i % 7, 120 + i % 5), (60, 60), (40, 200)]
+    Batch(fb, T, lens, 4 * hkv, hkv, hd, 16, 1, type).check(ref)
