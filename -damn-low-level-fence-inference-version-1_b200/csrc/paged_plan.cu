@@ -257,7 +257,8 @@ extern "C" int fence_paged_plan(const fence_paged_batch* b, fence_stream_t strea
     int grid = (int)((work + threads - 1) / threads);
     grid = grid < 1 ? 1 : grid > cap ? cap : grid;
     const int smem = (6 * b->n_req + 4) * (int)sizeof(int);
-    if (smem > 48 * 1024)
+    // a launch may use 48 KB without asking, the kernel's own arrays among them (48880 bytes were refused): ask well before
+    if (smem > 32 * 1024)
         FENCE_CUDA_TRY(cudaFuncSetAttribute(paged_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                             (6 * FENCE_PAGED_MAX_REQ + 4) * (int)sizeof(int)));
     return cuda_status(kv8_launch(paged_plan_kernel, dim3((unsigned)grid), threads, smem, (cudaStream_t)stream, p), "paged_plan");
