@@ -17,10 +17,15 @@
 //    so 8 query rows fill the instruction and nothing is padded for grouped heads. A page holds 16 or
 //    more keys: 16 keys share their scales. (A tile shared by the warps, 16 keys each, spent a third
 //    more instructions on the softmax state per key.)
-//  * Codes become fp16 exactly. Scales never touch them: k_scale multiplies the scores, v_scale / (the
-//    largest v_scale so far) the weights. q rows are brought to [256, 512) by a power of two, so that
-//    fp16 holds them whatever their range. SPLIT (fp32 activations): q and the weights as a pair of
-//    fp16 (22 bits), and the products of 16 keys are added to the sums in fp32 outside the matrix unit.
+//  * Codes become fp16 exactly. Scales never touch them: k_scale multiplies the scores, v_scale the
+//    weights. q rows are brought to [256, 512) by a power of two, so that fp16 holds them whatever their
+//    range. SPLIT (fp32 activations): q and the weights as a pair of fp16 (22 bits), and the products of
+//    16 keys are added to the sums in fp32 outside the matrix unit.
+//  * Two references per row, both of keys that the row sees: m for the sum of the weights, near the largest
+//    score s, and u for the sums of values, near the largest s + log2 v_scale. What is rounded to fp16 is
+//    2^(s - u + KD_UP) * v_scale: large where the row's own output comes from, whatever the scale of a page that it gives
+//    little weight (with the largest v_scale for a reference, pages 2^25 below it counted as zero). References are
+//    whole numbers: bringing sums to a new one is exact.
 #pragma once
 
 #include <cuda.h>
@@ -53,7 +58,9 @@ struct KAttnArgs {
 constexpr int KD_TILE = 32, KD_WARPS = 4, KD_THREADS = 32 * (KD_WARPS + 1);
 constexpr int KD_MIN_TILES = 4;  // tiles per CTA below which more CTAs only add joins
 constexpr int KD_UNIT = 8;       // a unit's start and end cost about as much as eight tiles: counted so when the runs are cut
-constexpr float KD_LAZY = 8.f;   // the running maximum may lag by 2^8: fp16 weights stay below 2^16
+constexpr float KD_LAZY = 8.f;   // the references may lag by 2^8
+constexpr float KD_UP = 6.f;     // weights enter fp16 times 2^6: below 2^(8 + 6 + 1), so small ones keep more of their bits
+constexpr float KD_FLOOR = 120.f;  // u >= m - 120, so that 2^(u - m) and its reciprocal are normal numbers: v_scale below that as if at it
 
 template <int HD, bool SPLIT, int NT>
 struct KDShape {
@@ -332,7 +339,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
         }
         named_bar_sync(1, 32 * KD_WARPS);
         // ---- this thread's rows 8 nt + 2 t + e: scale and last visible position
-        float qs[NT][2], m[NT][2], l[NT][2];
+        float qs[NT][2], m[NT][2], u[NT][2], l[NT][2];
         int lim[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -341,7 +348,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                 const int i = nt * 8 + 2 * t + e;
                 qs[nt][e] = s_qs[i] * a.scale_log2;
                 lim[nt][e] = i < rows ? q.kv - q.n + (row0 + i) / a.G : -1;
-                m[nt][e] = -INFINITY;
+                m[nt][e] = u[nt][e] = -INFINITY;
                 l[nt][e] = 0.f;
             }
         // keys that every row sees, and keys that some row sees
@@ -352,7 +359,6 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
-        float vref = 0.f, vinv = 0.f;
 
         for (int i = warp; i < cnt; i += KD_WARPS) {
             const uint32_t n = (uint32_t)(it + i);
@@ -414,16 +420,15 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                 }
                 // ---- scale, mask, the largest of each row
                 const bool masked = key0 + KD_TILE - 1 > lim_first || (a.window > 0 && key0 < all_lo);
-                float vmax = 0.f;
+                float lv[MK];  // whole part of log2 v_scale
 #pragma unroll
                 for (int y = 0; y < MK; ++y) {
                     // out of every row's sight the page was not fetched, nor its scales
                     if (masked && (key0 + y * 16 > lim_last || key0 + y * 16 + 15 < any_lo)) sv[y] = 0.f;
-                    if (sv[y] < INFINITY) vmax = fmaxf(vmax, sv[y]);
+                    lv[y] = sv[y] > 0.f && sv[y] < INFINITY ? (float)((int)(__float_as_uint(sv[y]) >> 23) - 127) : -INFINITY;
                 }
-                const bool grow = vmax > vref;
-                bool move = grow;
-                float mt[NT][2];
+                bool move = false;
+                float mt[NT][2], ut[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -444,59 +449,72 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                             }
                     }
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float x = fmaxf(acc[0][nt][e], acc[0][nt][e + 2]);
+                    for (int e = 0; e < 2; ++e) {  // this thread's keys; the whole row's only if a reference has to move
+                        float x = -INFINITY, w = -INFINITY;
 #pragma unroll
-                        for (int y = 1; y < MK; ++y) x = fmaxf(x, fmaxf(acc[y][nt][e], acc[y][nt][e + 2]));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                        for (int y = 0; y < MK; ++y) {
+                            const float z = fmaxf(acc[y][nt][e], acc[y][nt][e + 2]);
+                            x = fmaxf(x, z);
+                            w = fmaxf(w, z + lv[y]);
+                        }
                         mt[nt][e] = x;
-                        move |= x > m[nt][e] + KD_LAZY;  // also the first: m = -inf
+                        ut[nt][e] = w;
+                        move |= x > m[nt][e] + KD_LAZY || w > u[nt][e] + KD_LAZY;  // also the first: -inf
                     }
                 }
                 if (__any_sync(0xffffffffu, move)) {
-                    float vf = 1.f;
-                    if (grow) {
-                        vinv = 1.f / vmax;
-                        vf = vref * vinv;
-                        vref = vmax;
-                    }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float mn = fmaxf(m[nt][e], mt[nt][e]);
-                            const float al = mn == -INFINITY ? 1.f : kd_exp2(m[nt][e] - mn);
+                            float x = mt[nt][e], w = ut[nt][e];
+#pragma unroll
+                            for (int z = 4; z < 32; z *= 2) {
+                                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, z));
+                                w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, z));
+                            }
+                            // each row by itself: what another row sees has no say
+                            const float mn = x > m[nt][e] + KD_LAZY ? ceilf(x) : m[nt][e];
+                            const float un = fmaxf(w > u[nt][e] + KD_LAZY ? ceilf(w) : u[nt][e], mn - KD_FLOOR);
+                            l[nt][e] *= mn == -INFINITY ? 1.f : kd_exp2(m[nt][e] - mn);
+                            const float al = un == -INFINITY ? 1.f : kd_exp2(u[nt][e] - un);
                             m[nt][e] = mn;
-                            l[nt][e] *= al;
+                            u[nt][e] = un;
 #pragma unroll
                             for (int i2 = 0; i2 < MT; ++i2) {
-                                o[i2][nt][e] *= al * vf;
-                                o[i2][nt][e + 2] *= al * vf;
+                                o[i2][nt][e] *= al;
+                                o[i2][nt][e + 2] *= al;
                             }
                         }
                 }
-                // ---- the weights as B fragments, with the V scale over its reference
-                float mm[NT][2];
+                // ---- the weights as B fragments, with the V scale
+                float mm[NT][2], fu[NT][2];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) mm[nt][e] = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+                    for (int e = 0; e < 2; ++e) {
+                        mm[nt][e] = m[nt][e] == -INFINITY ? 0.f : m[nt][e];
+                        fu[nt][e] = m[nt][e] == -INFINITY ? 1.f : kd_exp2(KD_UP + m[nt][e] - u[nt][e]);
+                    }
                 uint32_t b0[MK][NT], b1[MK][NT], c0[SPLIT ? MK : 1][NT], c1[SPLIT ? MK : 1][NT];
 #pragma unroll
                 for (int y = 0; y < MK; ++y) {
                     // a NaN or infinite scale gives NaN to whoever sees the key
-                    const float fv = !(sv[y] < INFINITY) ? __uint_as_float(0x7fffffffu) : vref > 0.f ? sv[y] * vinv : 1.f;
-                    const bool apart = masked && !(fv < INFINITY);  // to nobody else
+                    if (!(sv[y] < INFINITY)) sv[y] = __uint_as_float(0x7fffffffu);
+                    const bool apart = masked && !(sv[y] < INFINITY);  // to nobody else
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float p[4];
+                        float p[4], fv[2];
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            fv[e] = sv[y] * fu[nt][e];
+                            if (fv[e] > 3e38f) fv[e] = 3e38f;  // a weight of 0 stays so; a NaN scale too
+                        }
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             const float x = kd_exp2(acc[y][nt][e] - mm[nt][e & 1]);
                             l[nt][e & 1] += x;
-                            p[e] = x * fv;
+                            p[e] = x * fv[e & 1];
                         }
                         if (apart) {
 #pragma unroll
@@ -572,7 +590,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
             if (lane == 0) mbar_arrive(&empty[s]);
         }
         it += cnt;
-        // ---- the four warps' results into one: largest m, then sum of o * v_ref * 2^(m - M)
+        // ---- the four warps' results into one: largest m, then sum of o * 2^(u - KD_UP - M)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -592,7 +610,7 @@ __global__ void __launch_bounds__(KD_THREADS, KDShape<HD, SPLIT, NT>::CTAS)
                 float M = -INFINITY;
 #pragma unroll
                 for (int w = 0; w < KD_WARPS; ++w) M = fmaxf(M, s_ml[w * ROWS + nt * 8 + 2 * t + e].x);
-                w_row[nt][e] = kd_exp2(m[nt][e] - (M == -INFINITY ? 0.f : M)) * vref;
+                w_row[nt][e] = exp2f(u[nt][e] - KD_UP - (M == -INFINITY ? 0.f : M));  // a power of 2, maybe a subnormal one
             }
         for (int w = 0; w < KD_WARPS; ++w) {
             if (w == warp) {

@@ -1,7 +1,7 @@
 // kv8_prefill.cuh — attention of many query rows per request over the paged 8-bit cache (prompts, chunks)
 // on the 5th-generation tensor cores.
 //
-//   S = Q . Kcode^T,  p = 2^(S * k_scale * scale * log2 e - m),  O = sum over keys of p * v_scale * Vcode,  out = O / sum p
+//   s = (Q . Kcode^T) * k_scale * scale * log2 e,  p = 2^(s - m),  O = sum over keys of p * v_scale * Vcode,  out = O / sum p
 //
 // Bound: the matrix unit (4 head_dim operations per visible pair) and, as large here, the exponentials:
 // 128 x 128 of them per tile at 16 a clock take as long as the tile's products. 2048 rows of 32 heads of 128 at 30000
@@ -18,7 +18,8 @@
 //  * Codes become fp16 exactly, once per tile for both streams, by four converter warps, from stages that
 //    TMA fills a tile ahead, and stored as they lie, keys by channels, in 128-byte swizzled shared
 //    memory: a K-major operand for S, an MN-major one for O. Scales never touch the codes: k_scale is
-//    part of a score's factor and v_scale / (a running reference) of the exponent, both constant over 16 keys.
+//    part of a score's factor and log2 v_scale of the exponent, both constant over 16 keys; the references of a
+//    row are its own, as in the decode kernel.
 //  * S, then P in its place as fp16 (the weights are the A operand straight from tensor memory), and O
 //    stay in tensor memory: 2 x (128 + head_dim) of its 512 columns.
 //  * O is rescaled only when a row's maximum grows by more than 2^8 (fp16 weights have that room).
@@ -598,10 +599,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                 __syncwarp();
                 if (lane < KT / 16) {
                     float lv = -INFINITY, rv = 1.f;
-                    if (vs > 0.f && vs < INFINITY) {
+                    if (vs >= 1.17549435e-38f && vs < INFINITY) {
                         lv = log2f(vs);
                         rv = 1.f / vs;
-                    } else if (vs != 0.f) {
+                    } else if (!(vs < INFINITY)) {
                         ks = __uint_as_float(0x7fffffffu);  // NaN for whoever sees these keys
                     }
                     float* d = s_prep + slot * 24;
@@ -735,7 +736,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const int r_lo = g.row0 + (SHARED ? 0 : 128 * s), r_hi = min(r_lo + 128, g.row0 + g.nrows) - 1;
             const int lim_first = g.q.kv - g.q.n + r_lo / a.G, lim_last = g.q.kv - g.q.n + r_hi / a.G;
             const float qs = valid ? a.q_scale[(long long)g.h * a.n_tokens * a.G + tok * a.G + (g.row0 + i_row) % a.G] : 1.f;
-            float m = -INFINITY, l = 0.f, lvref = -INFINITY, vref = 0.f;
+            // m, u: the row's references, as in the decode kernel; up = KD_UP + m - u, down = 2^-up
+            float m = -INFINITY, u = -INFINITY, l = 0.f, up = 0.f, down = 1.f;
             bool have_o = false;
             // the record of (CTA, slot, stream): m and l of each row, then the sums, four channels of all rows after one another
             auto record = [&]() { return a.part + ((long long)blockIdx.x * 4 + (g.first > 0 ? 0 : 2) + s) * S::REC; };
@@ -760,8 +762,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                             v.x *= f, v.y *= f, v.z *= f, v.w *= f;
                         }
                         if (have_o) {
-                            v.x = fmaf(__uint_as_float(r[e]), vref, v.x), v.y = fmaf(__uint_as_float(r[e + 1]), vref, v.y);
-                            v.z = fmaf(__uint_as_float(r[e + 2]), vref, v.z), v.w = fmaf(__uint_as_float(r[e + 3]), vref, v.w);
+                            v.x = fmaf(__uint_as_float(r[e]), down, v.x), v.y = fmaf(__uint_as_float(r[e + 1]), down, v.y);
+                            v.z = fmaf(__uint_as_float(r[e + 2]), down, v.z), v.w = fmaf(__uint_as_float(r[e + 3]), down, v.w);
                         }
                         __stcg(at, v);
                     }
@@ -821,7 +823,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     return f;
                 };
                 constexpr int CH = 32, NB = CH / 16;
-                float mt = -INFINITY, lvmax = -INFINITY;
+                float mt = -INFINITY, ut = -INFINITY;
 #pragma unroll 1
                 for (int c = 0; c < KT; c += CH) {
                     uint32_t x[CH];
@@ -829,30 +831,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
                     float f[NB];
 #pragma unroll
-                    for (int k = 0; k < NB; ++k) {
-                        f[k] = factor(c / 16 + k);
-                        lvmax = fmaxf(lvmax, pr[8 + c / 16 + k]);
-                    }
+                    for (int k = 0; k < NB; ++k) f[k] = factor(c / 16 + k);
                     kp_wait_ld();
 #pragma unroll
                     for (int k = 0; k < NB; ++k) {
                         float y = __uint_as_float(x[16 * k]);
 #pragma unroll
                         for (int e = 1; e < 16; ++e) y = fmaxf(y, __uint_as_float(x[16 * k + e]));
-                        mt = fmaxf(mt, y * f[k]);
+                        y *= f[k];
+                        mt = fmaxf(mt, y);
+                        ut = fmaxf(ut, y + pr[8 + c / 16 + k]);
                     }
                 }
-                const bool move_v = lvmax > lvref + 4.f;
-                if (__any_sync(0xffffffffu, move_v || mt > m + KD_LAZY)) {
-                    const float mn = fmaxf(m, mt), lvn = move_v ? lvmax : lvref;
-                    float al = mn == -INFINITY ? 1.f : kd_exp2(m - mn);
-                    l *= al;
-                    if (move_v) {
-                        al *= lvref == -INFINITY ? 0.f : kd_exp2(lvref - lvn);
-                        lvref = lvn;
-                        vref = exp2f(lvn);
-                    }
-                    m = mn;
+                if (__any_sync(0xffffffffu, mt > m + KD_LAZY || ut > u + KD_LAZY)) {
+                    // each row by itself: what another row sees has no say
+                    const float mn = mt > m + KD_LAZY ? ceilf(mt) : m;
+                    const float un = fmaxf(ut > u + KD_LAZY ? ceilf(ut) : u, mn - KD_FLOOR);
+                    l *= mn == -INFINITY ? 1.f : kd_exp2(m - mn);
+                    const float al = un == -INFINITY ? 1.f : kd_exp2(u - un);
+                    m = mn, u = un;
+                    up = m == -INFINITY ? 0.f : KD_UP + m - u;
+                    down = kd_exp2(-up);
                     if (have_o) {  // the products of the tiles before have ended: S came after them
 #pragma unroll 1
                         for (int c = 0; c < HDO; c += 16) {
@@ -866,7 +865,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                     }
                 }
                 have_o = true;
-                const float mm = m == -INFINITY ? 0.f : m, lv0 = lvref == -INFINITY ? 0.f : lvref;
+                const float mm = m == -INFINITY ? 0.f : m;
                 // ---- weights, in place of the scores
 #pragma unroll 1
                 for (int c = 0; c < KT; c += CH) {
@@ -877,13 +876,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
 #pragma unroll
                     for (int k = 0; k < NB; ++k) {
                         const int b = c / 16 + k;
-                        const float d = pr[8 + b] - lv0;
-                        const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it
+                        const float d = pr[8 + b] + up;
+                        const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it for this row
                         cf[k] = factor(b);
                         add[k] = SPLIT ? -mm : (tiny ? -40.f : d) - mm;
                         if ((bad >> b) & 1u) add[k] = __uint_as_float(0x7fffffffu);
-                        fb[k] = SPLIT ? (tiny ? 0.f : kd_exp2(d)) : 0.f;
-                        fl[k] = SPLIT ? 1.f : tiny ? 1.0995116e12f : pr[16 + b] * (lvref == -INFINITY ? 1.f : vref);
+                        fb[k] = SPLIT ? (tiny ? 0.f : kd_exp2(fminf(d, 127.f))) : 0.f;
+                        fl[k] = SPLIT ? 1.f : tiny ? 1.0995116e12f : pr[16 + b] * down;
                     }
                     kp_wait_ld();
 #pragma unroll
@@ -929,7 +928,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             if (SPLIT) {
                 drain();
             } else {  // out, or to the record
-                const float mul = direct ? (l == 0.f ? 0.f : vref / l) : vref;
+                const float mul = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
                 float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
 #pragma unroll 1
                 for (int c = 0; c < HDO; c += 16) {
@@ -940,7 +939,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         kp_wait_ld();
                     }
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) x[e] = have_o && mul != 0.f ? __uint_as_float(r[e]) * mul : 0.f;
+                    for (int e = 0; e < 16; ++e) x[e] = have_o && mul != 0.f ? __uint_as_float(r[e]) * mul * down : 0.f;
                     if (direct) {
                         const long long at = tok * a.out_stride + (long long)head * HD + ch0 + c;
                         if (valid) {

@@ -511,7 +511,9 @@ typedef struct fence_kv8_attn {
  * through block_table[r]. Uses b->n_req, n_tokens, max_pages, block_table, kv_len and new_start. Rows
  * that see nothing (a request that is not placed, rows after the last request's) give 0 and lse -inf.
  * Codes enter the products exactly, q and the softmax weights as fp16 (fp32 q: as a pair of fp16);
- * sums are fp32. The result does not depend on timing. Calls that overlap in time need workspaces of
+ * sums are fp32. Weights are rounded relative to what their row sees, V scales included: a page's scale
+ * may differ from the others' by any factor, and keys out of a row's sight do not change its bits. The
+ * result does not depend on timing. Calls that overlap in time need workspaces of
  * their own. */
 size_t fence_kv8_attention_workspace_bytes(const fence_kv8_cache* c, const fence_paged_batch* b,
                                            const fence_kv8_attn* a);
