@@ -159,8 +159,10 @@ extern "C" int fence_kv8_attention(const fence_kv8_cache* c, const fence_paged_b
     const size_t need = fence_kv8_attention_workspace_bytes(c, b, a);
     if (a->workspace_bytes < need)
         return set_error(FENCE_E_SCRATCH, "kv8_attention: workspace of %zu bytes, needs %zu", a->workspace_bytes, need);
+    // a window as long as any request is none; positions less a window (at most 2^30 each) stay within 32 bits
+    const int window = a->window > 0 && a->window < (long long)b->max_pages * b->page_tokens ? a->window : 0;
     KAttnArgs p{*c, b->block_table, b->kv_len, b->new_start, b->n_req, b->n_tokens, b->max_pages, ilog2(c->page_tokens),
-                a->n_q_heads / c->n_kv_heads, a->n_q_heads, a->window > 0 ? a->window : 0, a->type, a->q, a->out, a->lse,
+                a->n_q_heads / c->n_kv_heads, a->n_q_heads, window, a->type, a->q, a->out, a->lse,
                 a->q_stride, a->out_stride, (float)(a->scale * 1.4426950408889634), INT_MAX, 0, 0, kv8_wide(a->q, a->q_stride, a->type),
                 kv8_wide(a->out, a->out_stride, a->type), nullptr, nullptr, static_cast<int*>(a->workspace),
                 reinterpret_cast<float*>(static_cast<char*>(a->workspace) + KV8_ARRIVED_BYTES)};

@@ -44,3 +44,18 @@ def test_rows_before_the_first_position(fb, T, ref, hkv, hd, type):  # noqa: F81
     for i in range(120 // hkv):
         lens += [(50 + i % 7, 120 + i % 5), (60, 60), (40, 200)]
     Batch(fb, T, lens, 4 * hkv, hkv, hd, 16, 1, type).check(ref)
+
+
+@pytest.mark.parametrize("n", [1, 5, 60])
+@pytest.mark.parametrize("type", [0, 2])
+def test_windows_longer_than_any_request(fb, T, ref, n, type):  # noqa: F811
+    """Up to the largest int the window hides nothing, with requests that are not placed or have more rows than positions."""
+    b = Batch(fb, T, [(500, n), (0, n + 2), (max(1, n - 3), n), (40, 200 if n == 60 else n)], 8, 2, 128, 16, 0, type)
+    b.check(ref)
+    want = [x.clone() for x in b.run()]
+    for window in (2 ** 31 - 1, 2 ** 31 - 64, 2 ** 30, 16 * b.max_pages, 16 * b.max_pages - 1):
+        b.window = window
+        for x in (b.out, b.lse):
+            x.fill_(7)
+        got = b.run()
+        assert T.equal(got[0], want[0]) and T.equal(got[1], want[1])
