@@ -579,12 +579,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const KPSeg g = walk.seek(a, cur, end);
             if (g.cnt <= 0) break;
             const int* table = a.block_table + (size_t)walk.r * a.max_pages;
+            // the first key that some row of the unit sees: pages before it may be anyone's by now
+            const int any_lo = a.window > 0 ? max(0, g.q.kv - g.q.n + g.row0 / a.G - a.window + 1) : 0;
             for (int j = 0; j < g.cnt; ++j) {
                 const int kt = g.tile0 + j, key = kt * KT + lane * 16;
                 if (!kp_active<SPLIT>(g, 0, kt) && !kp_active<SPLIT>(g, 1, kt)) continue;
                 int unit = 0;
                 float ks = 0.f, vs = 0.f;
-                if (lane < KT / 16 && key < g.q.kv) {
+                if (lane < KT / 16 && key < g.q.kv && (key | (a.c.page_tokens - 1)) >= any_lo) {
                     int p = table[key >> a.shift];
                     if (p < 0 || p >= a.c.n_pages) {
                         set_device_error(KV8_BAD);

@@ -508,7 +508,8 @@ typedef struct fence_kv8_attn {
 
 /* Causal grouped-query attention of the batch: of request r's n = new_start[r+1] - new_start[r] rows,
  * row i is at position kv_len[r] - n + i and sees the positions 0 .. that one (the last `window`)
- * through block_table[r]. Uses b->n_req, n_tokens, max_pages, block_table, kv_len and new_start. Rows
+ * through block_table[r]. Uses b->n_req, n_tokens, max_pages, block_table, kv_len and new_start; table
+ * entries of pages wholly before the window of the request's first row are not used. Rows
  * that see nothing (a request that is not placed, rows after the last request's) give 0 and lse -inf.
  * Codes enter the products exactly, q and the softmax weights as fp16 (fp32 q: as a pair of fp16);
  * sums are fp32. Weights are rounded relative to what their row sees, V scales included: a page's scale

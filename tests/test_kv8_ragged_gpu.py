@@ -59,3 +59,17 @@ def test_windows_longer_than_any_request(fb, T, ref, n, type):  # noqa: F811
             x.fill_(7)
         got = b.run()
         assert T.equal(got[0], want[0]) and T.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("n", [1, 5, 60, 300])
+@pytest.mark.parametrize("hd,type", [(64, 0), (128, 1), (256, 2)])
+@pytest.mark.parametrize("page", [16, 64])
+def test_table_entries_before_the_window_are_not_used(fb, T, ref, n, hd, type, page):  # noqa: F811
+    """Pages that the window has left behind may be given away: their entries in the table hold no page."""
+    b = Batch(fb, T, [(900, n), (500, n)], 8, 2, hd, page, 0, type, window=70)
+    want = [x.clone() for x in b.run()]
+    for r, (kv, m) in enumerate(b.lens):
+        b.d_table[r, :max(0, kv - m + 1 - 70) // page] = -1
+    got = b.run()
+    assert fb.lib().fence_device_error() == 0
+    assert T.equal(got[0], want[0]) and T.equal(got[1], want[1])
