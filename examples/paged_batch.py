@@ -1,9 +1,9 @@
 """Several requests served at once over a paged 8-bit KV cache: prompts of different lengths enter while others decode,
-requests end and give their pages back.
+requests end and give their pages back; what does not fit comes again.
 
 A small attention-only decoder with random weights stands in for a model: per layer the q|k|v projection
 (fence_gemm_f16), rotary embedding, fence_kv8_store, fence_kv8_attention and the output projection. One
-fence_paged_plan per step serves all layers; nothing of a step's lengths is read back to the host.
+fence_paged_plan per step serves all layers; a step copies its greedy ids and kv_len to the host, once.
 
     python examples/paged_batch.py
 """
@@ -36,7 +36,7 @@ class Decoder:
     def __init__(self, layers=2, hq=8, hkv=2, hd=64, vocab=512, n_pages=64, page=16, max_req=8, max_pages=16, max_tokens=256, fmt=None, seed=0):
         g = torch.Generator(device="cuda").manual_seed(seed)
         rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
-        self.layers, self.hq, self.hkv, self.hd, self.page, self.dim = layers, hq, hkv, hd, page, hq * hd
+        self.layers, self.hq, self.hkv, self.hd, self.page, self.dim, self.max_tokens = layers, hq, hkv, hd, page, hq * hd, max_tokens
         self.embed = rnd(vocab, self.dim).half()
         self.wqkv = [(rnd((hq + 2 * hkv) * hd, self.dim) * self.dim ** -0.5).half() for _ in range(layers)]
         self.wo = [(rnd(self.dim, self.dim) * self.dim ** -0.5).half() for _ in range(layers)]
@@ -84,6 +84,8 @@ class Decoder:
         """One step: new_len[r] tokens of request r (0: waits, -1: has ended), `tokens` one after another. Returns the
         logits of every token row."""
         T, b, a = len(tokens), self.batch, self.attn
+        if T > self.max_tokens:
+            raise ValueError("%d tokens in a step of at most %d" % (T, self.max_tokens))
         self.stream = torch.cuda.current_stream().cuda_stream
         self.new_len.copy_(torch.tensor(new_len, dtype=torch.int32))
         b.n_tokens = T
@@ -111,35 +113,68 @@ class Decoder:
 
 
 def serve(dec, prompts, max_new=12, arrive_every=2):
-    """Greedy decoding of all prompts; a prompt enters a free row every few steps. Returns the generated ids per prompt."""
-    rows = [None] * dec.batch.n_req  # the prompt index that a row serves
+    """Greedy decoding of all prompts; a prompt enters a free row every few steps. Returns the generated ids per prompt.
+
+    A step sends at most max_tokens rows, so a long prompt goes in chunks. A request that the plan could not place brings the
+    same tokens again, and none enters meanwhile. Where nothing could be placed, the request that entered last gives its
+    pages back and starts over later, with what it has generated as part of its prompt."""
+    b = dec.batch
+    longest = min(b.max_pages, b.n_pages) * b.page_tokens
+    for p in prompts:
+        if not p or len(p) + max_new - 1 > longest:
+            raise ValueError("a prompt of %d tokens with %d new ones: at least 1 and at most %d fit" % (len(p), max_new, longest))
+    rows = [None] * b.n_req  # the prompt index that a row serves
     out, waiting, step = [[] for _ in prompts], list(range(len(prompts))), 0
-    ended = []
-    while waiting or any(r is not None for r in rows) or ended:
-        new_len, tokens, last = [0] * len(rows), [], {}
+    due = [list(p) for p in prompts]  # what each request has still to bring
+    entered, ended = [], []  # rows in the order in which they were taken; rows whose request has ended
+    short = False  # not all could be placed
+    while waiting or entered or ended:
+        new_len, tokens, sent = [0] * len(rows), [], {}
         for r in ended:
             new_len[r] = -1
-        if waiting and step % arrive_every == 0:
+        if waiting and step % arrive_every == 0 and not short:
             free = [r for r, p in enumerate(rows) if p is None and r not in ended]
             if free:
                 rows[free[0]] = waiting.pop(0)
+                entered.append(free[0])
         for r, p in enumerate(rows):
-            if p is None or new_len[r] < 0:
+            if p is None:
                 continue
-            ids = prompts[p] if not out[p] else out[p][-1:]
+            ids = due[p][:dec.max_tokens - len(tokens)]
             new_len[r] = len(ids)
-            tokens += ids
-            last[r] = len(tokens) - 1
-        ended = []
+            if ids:
+                tokens += ids
+                sent[r] = len(tokens) - 1
+        freed, ended = bool(ended), []
         logits = dec.step(new_len, tokens, max([1] + new_len))
-        if last:
-            ids = logits[list(last.values())].argmax(-1).tolist()  # the step's only copy to the host
-            for r, t in zip(last, ids):
-                out[rows[r]].append(t)
-                if len(out[rows[r]]) == max_new:
-                    rows[r] = None
-                    ended.append(r)
         step += 1
+        if not sent:
+            short = False
+            continue
+        # the step's only copy to the host: the greedy ids, and which requests were placed
+        got = torch.cat([logits[list(sent.values())].argmax(-1).int(), dec.kv_len[list(sent)]]).tolist()
+        placed = 0
+        for r, t, kv in zip(sent, got, got[len(sent):]):
+            if kv == 0:
+                continue
+            placed += 1
+            p = rows[r]
+            due[p] = due[p][new_len[r]:]
+            if due[p]:
+                continue  # more of its prompt to come
+            out[p].append(t)
+            due[p] = [t]
+            if len(out[p]) == max_new:
+                rows[r] = None
+                entered.remove(r)
+                ended.append(r)
+        short = placed < len(sent)
+        if not placed and not freed:
+            r = entered.pop()
+            waiting.insert(0, rows[r])
+            due[rows[r]] = prompts[rows[r]] + out[rows[r]]
+            rows[r] = None
+            ended.append(r)
     return out
 
 
