@@ -64,10 +64,12 @@ constexpr float KD_FLOOR = 120.f;  // u >= m - 120, so that 2^(u - m) and its re
 
 template <int HD, bool SPLIT, int NT>
 struct KDShape {
-    // CTAs per SM, by the registers that the sums take
-    static constexpr int CTAS = HD == 256 ? (NT == 2 ? 1 : 2) : (HD == 128 && NT == 2 ? 2 : 3);
+    // CTAs per SM, by the registers that the sums take (256 channels of fp32: 103 us with one, 109 with the registers of two, 4
+    // requests of 30000 to 60000 keys)
+    static constexpr int CTAS = HD == 256 ? (NT == 2 || SPLIT ? 1 : 2) : (HD == 128 && NT == 2 ? 2 : 3);
     // twice as many stages as warps: with one each, every tile's load began when the tile before it was done with
-    static constexpr int STAGES = HD == 64 ? 12 : HD == 128 ? (CTAS == 3 ? 8 : 12) : NT == 2 ? 10 : 6;
+    // (SPLIT's second part of q takes the place of one: with 12 a single CTA fitted, 47 us against 37 for drafts of 4)
+    static constexpr int STAGES = HD == 64 ? 12 : HD == 128 ? (CTAS == 3 ? 8 : SPLIT ? 11 : 12) : CTAS == 1 ? 10 : 6;
     static constexpr int KV_BYTES = KD_TILE * HD;
     static constexpr int STAGE = 2 * KV_BYTES;
     static constexpr int ROWS = 8 * NT;
@@ -81,6 +83,7 @@ struct KDShape {
     static constexpr int O_SLAB = O_ML + KD_WARPS * ROWS * 8;
     static constexpr int O_SCAN = O_SLAB + ROWS * SLAB * 4;
     static constexpr int SMEM = O_SCAN + 64 + 1024;  // + the prefix sums [n_req + 1], + alignment
+    static_assert(CTAS * (SMEM + 4 * 257 + 1024) <= 228 * 1024, "CTAS of them fit an SM, for up to 256 requests");
 };
 
 __device__ __forceinline__ void kd_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
