@@ -58,40 +58,8 @@ __device__ __forceinline__ uint32_t kd_half2(uint32_t w, bool high) {
 template <int FMT>
 __device__ __forceinline__ uint32_t kd_bias(uint32_t w) { return FMT == KV8_INT8 ? w ^ 0x80808080u : w; }
 
-// 8 consecutive elements of a row of activations. `wide`: the row is 16-byte aligned.
-__device__ __forceinline__ void kv8_ld8(const void* base, long long i, int type, bool wide, float (&x)[8]) {
-    if (type == FENCE_F32) {
-        const float* p = static_cast<const float*>(base) + i;
-        if (wide) {
-            const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = p[j];
-        }
-        return;
-    }
-    uint32_t w[4];
-    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
-    if (wide) {
-        const uint4 a = *reinterpret_cast<const uint4*>(p);
-        w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-    } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = (uint32_t)p[2 * j] | ((uint32_t)p[2 * j + 1] << 16);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (type == FENCE_F16) {
-            x[2 * j] = half_bits_to_float(w[j]);
-            x[2 * j + 1] = half_bits_to_float(w[j] >> 16);
-        } else {
-            x[2 * j] = __uint_as_float(w[j] << 16);
-            x[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-        }
-    }
-}
-// The same with the type known: 16 raw bytes per 8 elements of 16 bits, 32 per 8 floats, and their values.
+// 8 consecutive elements of a row of activations, raw: 16 bytes of 16-bit types, 32 of floats (WIDE: the row is 16-byte aligned),
+// and their values.
 template <int TYPE, bool WIDE>
 __device__ __forceinline__ void kv8_raw8(const void* base, long long i, uint32_t (&w)[TYPE == FENCE_F32 ? 8 : 4]) {
     if (TYPE == FENCE_F32) {

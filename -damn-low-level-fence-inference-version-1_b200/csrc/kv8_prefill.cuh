@@ -25,8 +25,6 @@
 //  * O is rescaled only when a row's maximum grows by more than 2^8 (fp16 weights have that room).
 #pragma once
 
-#include <type_traits>
-
 #include "kv8_decode.cuh"
 
 namespace fence {
