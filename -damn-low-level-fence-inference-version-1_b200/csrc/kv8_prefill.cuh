@@ -33,9 +33,11 @@ constexpr int KP_SMS = 148;
 constexpr int KP_W_CONV = 8, KP_W_PREP = 12, KP_W_MMA = 13, KP_W_LOAD = 14, KP_THREADS = 480;
 constexpr int KP_MIN_TILES = 2, KP_SLOTS = 4;
 constexpr int KP_UNIT = 4;  // a unit's start and end cost about as much as four tiles: counted so when the runs are cut
-// SPLIT: the matrix unit's additions cut the sum's last bit off, half of it on average and always towards zero: 128 of
-// them (8 tiles) cost 2e-6. So after every 4 tiles of a stream the sums are added, rounded, to the stream's record.
-constexpr int KP_DRAIN = 4;
+// The matrix unit's additions cut the sum's last bit off, half of it on average and always towards zero: 128 of them (8
+// tiles) cost 2e-6, 30000 keys 1.2e-4, and 131000 keys in one go 7e-4, more than fp16's rounding (2^-12 at least). So the sums are
+// added, rounded, to the stream's record from time to time: every 4 tiles of a stream for fp32 activations, every
+// KP_TURN_KEYS keys for 16 bits (every 8192 keys took 1382 us where this takes 1280, 2048 rows at 30000 keys).
+constexpr int KP_TURN_SPLIT = 4, KP_TURN_KEYS = 32768;
 
 template <int HD, bool SPLIT>
 struct KPShape {
@@ -55,6 +57,8 @@ struct KPShape {
     static constexpr int O_MISC = O_BAR + 256;
     static constexpr int O_PREP = O_MISC + 64;  // [KP_SLOTS][24]: k_scale, log2 v_scale, 1 / v_scale of 8 x 16 keys; [KP_SLOTS][8]: the pool's row of their first
     static constexpr int SMEM = O_PREP + KP_SLOTS * 128 + 1024;
+    // tiles between two times; the first of a stream after one is among the next STEP
+    static constexpr int STEP = SPLIT ? 2 : 1, TURN = SPLIT ? 2 * KP_TURN_SPLIT : KP_TURN_KEYS / KT;
     static constexpr int REC = 128 * (HDO + 2);  // floats of one stream's partial result
 };
 
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             const KPSeg g = walk.seek(a, cur, end);
             if (g.cnt <= 0) break;
             int pend0 = -1, pend1 = -1;      // the tile (count) whose weights a stream is making
-            uint32_t have = 0, left = 0, made[2] = {0, 0};  // have: q (bits 0, 1) and o (2, 3) of the streams; left: streams that still need V, 8 bits per buffer
+            uint32_t have = 0, left = 0;  // have: q (bits 0, 1) and o (2, 3) of the streams; left: streams that still need V, 8 bits per buffer
             const int last = g.tile0 + g.cnt;
             // one more round than tiles, two where the streams take turns, to finish the last weights
             for (int kt = g.tile0; kt < last + (SPLIT ? 2 : 1); ++kt) {
@@ -643,13 +647,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         wait(&p_full[s], np >> (16 * s));
                         np ^= 1u << (16 * s);
                         left -= 1u << (8 * pb);
-                        uint32_t add = (have >> (2 + s)) & 1u;
+                        const uint32_t add = (have >> (2 + s)) & (uint32_t)((kt - S::STEP - g.tile0) % S::TURN >= S::STEP);
                         have |= 4u << s;
-                        if (SPLIT) {
-                            add = (s ? made[1] : made[0]) % KP_DRAIN != 0;
-                            if (s) ++made[1];
-                            else ++made[0];
-                        }
                         kp_fence_after();
                         const uint32_t d = __shfl_sync(0xffffffffu, tm + 256 + 128 * s, 0), ta = __shfl_sync(0xffffffffu, tm + 128 * s, 0);
                         const uint64_t db = kp_desc_mn(__shfl_sync(0xffffffffu, sbase + S::O_V + pb * S::OP + (HALVES ? s * 2 * KT * 128 : 0), 0), KT * 128);
@@ -741,195 +740,172 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
             bool have_o = false;
             // the record of (CTA, slot, stream): m and l of each row, then the sums, four channels of all rows after one another
             auto record = [&]() { return a.part + ((long long)blockIdx.x * 4 + (g.first > 0 ? 0 : 2) + s) * S::REC; };
-            float m_rec = -INFINITY;  // SPLIT: what the record's sums so far are relative to
-            int since = 0, drained = 0;
-            auto drain = [&]() {  // the sums to the record
-                const float f = drained ? kd_exp2(m_rec - (m == -INFINITY ? 0.f : m)) : 0.f;
-                float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
-#pragma unroll 1
-                for (int c = 0; c < HDO; c += 16) {
-                    uint32_t r[16];
-                    if (have_o) {
-                        KP_LD16(r, t_o + c);
-                        kp_wait_ld();
+            const bool whole = g.cnt == g.tiles, direct = whole && !SPLIT && g.cnt <= S::TURN;  // the same for both streams
+            bool again = false;  // the record holds sums already
+            for (int j = 0;;) {
+                for (const int stop = min(g.cnt, j + S::TURN); j < stop; ++j) {
+                    const int kt = g.tile0 + j, key0 = kt * KT;
+                    const bool act = kp_active<SPLIT>(g, s, kt);
+                    if (!act && !kp_active<SPLIT>(g, 1 - s, kt)) continue;
+                    const uint32_t slot = it % KP_SLOTS, use = it / KP_SLOTS;
+                    ++it;
+                    wait(&prep_full[slot], use);  // also where this stream has no rows: it must not give back a slot before its time
+                    __syncwarp();
+                    if (!act) {
+                        if (lane == 0) mbar_arrive(&prep_empty[slot]);
+                        continue;
                     }
-#pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        float4* at = rec + ((c + e) >> 2) * 128;
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (SPLIT && drained) {
-                            v = __ldcg(at);
-                            v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-                        }
-                        if (have_o) {
-                            v.x = fmaf(__uint_as_float(r[e]), down, v.x), v.y = fmaf(__uint_as_float(r[e + 1]), down, v.y);
-                            v.z = fmaf(__uint_as_float(r[e + 2]), down, v.z), v.w = fmaf(__uint_as_float(r[e + 3]), down, v.w);
-                        }
-                        __stcg(at, v);
-                    }
-                }
-                drained = 1;
-                m_rec = m;
-            };
-            for (int j = 0; j < g.cnt; ++j) {
-                const int kt = g.tile0 + j, key0 = kt * KT;
-                const bool act = kp_active<SPLIT>(g, s, kt);
-                if (!act && !kp_active<SPLIT>(g, 1 - s, kt)) continue;
-                const uint32_t slot = it % KP_SLOTS, use = it / KP_SLOTS;
-                ++it;
-                wait(&prep_full[slot], use);  // also where this stream has no rows: it must not give back a slot before its time
-                __syncwarp();
-                if (!act) {
-                    if (lane == 0) mbar_arrive(&prep_empty[slot]);
-                    continue;
-                }
-                wait(&s_full[s], n_s++);
-                __syncwarp();
-                kp_fence_after();
-                if (SPLIT && since == KP_DRAIN) {  // the products of the tiles before have ended: S came after them
-                    drain();
-                    since = 0;
-                    have_o = false;
-                    kp_fence_before();
-                }
-                if (SPLIT) ++since;
-                const float* pr = s_prep + slot * 24;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
-                // Loops of 32 columns, not unrolled: the roles' code has to share the instruction cache.
-                const bool edge = key0 + KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
-                uint32_t bad = 0;  // of an edge tile: blocks of 16 keys with a scale that is no number, of which this row sees some
-                if (edge) {        // -infinity in the columns that this row does not see
+                    wait(&s_full[s], n_s++);
+                    __syncwarp();
+                    kp_fence_after();
+                    const float* pr = s_prep + slot * 24;  // k_scale, log2 and reciprocal of v_scale of 8 x 16 keys
+                    // Loops of 32 columns, not unrolled: the roles' code has to share the instruction cache.
+                    const bool edge = key0 + KT - 1 > lim_first || (a.window > 0 && key0 < lim_last - a.window + 1);
+                    uint32_t bad = 0;  // of an edge tile: blocks of 16 keys with a scale that is no number, of which this row sees some
+                    if (edge) {        // -infinity in the columns that this row does not see
 #pragma unroll 1
-                    for (int c = 0; c < KT / 32; ++c) {
-                        uint32_t x[32];
-                        KP_LD32(x, t_s + 32 * c);
-                        kp_wait_ld();
-                        const int h = lim - key0 - 32 * c, l0 = lim_lo - key0 - 32 * c;  // sees the columns l0 .. h
-                        uint32_t see = h < 0 ? 0u : h >= 31 ? ~0u : (2u << h) - 1u;
-                        if (l0 > 0) see &= l0 >= 32 ? 0u : ~0u << l0;
+                        for (int c = 0; c < KT / 32; ++c) {
+                            uint32_t x[32];
+                            KP_LD32(x, t_s + 32 * c);
+                            kp_wait_ld();
+                            const int h = lim - key0 - 32 * c, l0 = lim_lo - key0 - 32 * c;  // sees the columns l0 .. h
+                            uint32_t see = h < 0 ? 0u : h >= 31 ? ~0u : (2u << h) - 1u;
+                            if (l0 > 0) see &= l0 >= 32 ? 0u : ~0u << l0;
 #pragma unroll
-                        for (int e = 0; e < 32; ++e)
-                            if (!((see >> e) & 1u)) x[e] = 0xff800000u;
-                        KP_ST16(t_s + 32 * c, x);
-                        KP_ST16(t_s + 32 * c + 16, (x + 16));
-                        if (!(pr[2 * c] * qs < INFINITY) && (see & 0xffffu)) bad |= 1u << (2 * c);
-                        if (!(pr[2 * c + 1] * qs < INFINITY) && (see >> 16)) bad |= 2u << (2 * c);
+                            for (int e = 0; e < 32; ++e)
+                                if (!((see >> e) & 1u)) x[e] = 0xff800000u;
+                            KP_ST16(t_s + 32 * c, x);
+                            KP_ST16(t_s + 32 * c + 16, (x + 16));
+                            if (!(pr[2 * c] * qs < INFINITY) && (see & 0xffffu)) bad |= 1u << (2 * c);
+                            if (!(pr[2 * c + 1] * qs < INFINITY) && (see >> 16)) bad |= 2u << (2 * c);
+                        }
+                        kp_wait_st();
+                    }
+                    // factor of a block's scores; -infinity has to stay so in an edge tile: none of 0 or NaN there
+                    auto factor = [&](int b) {
+                        float f = pr[b] * qs;
+                        if (edge) f = f < INFINITY ? fmaxf(f, 1e-30f) : 1e-30f;
+                        return f;
+                    };
+                    constexpr int CH = 32, NB = CH / 16;
+                    float mt = -INFINITY, ut = -INFINITY;
+#pragma unroll 1
+                    for (int c = 0; c < KT; c += CH) {
+                        uint32_t x[CH];
+#pragma unroll
+                        for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
+                        float f[NB];
+#pragma unroll
+                        for (int k = 0; k < NB; ++k) f[k] = factor(c / 16 + k);
+                        kp_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < NB; ++k) {
+                            float y = __uint_as_float(x[16 * k]);
+#pragma unroll
+                            for (int e = 1; e < 16; ++e) y = fmaxf(y, __uint_as_float(x[16 * k + e]));
+                            y *= f[k];
+                            mt = fmaxf(mt, y);
+                            ut = fmaxf(ut, y + pr[8 + c / 16 + k]);
+                        }
+                    }
+                    if (__any_sync(0xffffffffu, mt > m + KD_LAZY || ut > u + KD_LAZY)) {
+                        // each row by itself: what another row sees has no say
+                        const float mn = mt > m + KD_LAZY ? ceilf(mt) : m;
+                        const float un = fmaxf(ut > u + KD_LAZY ? ceilf(ut) : u, mn - KD_FLOOR);
+                        l *= mn == -INFINITY ? 1.f : kd_exp2(m - mn);
+                        const float al = un == -INFINITY ? 1.f : kd_exp2(u - un);
+                        m = mn, u = un;
+                        up = m == -INFINITY ? 0.f : KD_UP + m - u;
+                        down = kd_exp2(-up);
+                        if (have_o) {  // the products of the tiles before have ended: S came after them
+#pragma unroll 1
+                            for (int c = 0; c < HDO; c += 16) {
+                                uint32_t r[16];
+                                KP_LD16(r, t_o + c);
+                                kp_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * al);
+                                KP_ST16(t_o + c, r);
+                            }
+                        }
+                    }
+                    have_o = true;
+                    const float mm = m == -INFINITY ? 0.f : m;
+                    // ---- weights, in place of the scores
+#pragma unroll 1
+                    for (int c = 0; c < KT; c += CH) {
+                        uint32_t x[CH];
+#pragma unroll
+                        for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
+                        float cf[NB], add[NB], fb[NB], fl[NB];
+#pragma unroll
+                        for (int k = 0; k < NB; ++k) {
+                            const int b = c / 16 + k;
+                            const float d = pr[8 + b] + up;
+                            const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it for this row
+                            cf[k] = factor(b);
+                            add[k] = SPLIT ? -mm : (tiny ? -40.f : d) - mm;
+                            if ((bad >> b) & 1u) add[k] = __uint_as_float(0x7fffffffu);
+                            fb[k] = SPLIT ? (tiny ? 0.f : kd_exp2(fminf(d, 127.f))) : 0.f;
+                            fl[k] = SPLIT ? 1.f : tiny ? 1.0995116e12f : pr[16 + b] * down;
+                        }
+                        kp_wait_ld();
+#pragma unroll
+                        for (int h = 0; h < CH / 32; ++h) {
+                            uint32_t hi[16], lo[16];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int kb = 2 * h + k;
+                                const uint64_t cf2 = kp_two(cf[kb], cf[kb]), add2 = kp_two(add[kb], add[kb]);
+                                uint64_t sum2 = 0;
+#pragma unroll
+                                for (int e = 0; e < 16; e += 2) {
+                                    const float2 y = kp_both(kp_fma2(
+                                        kp_two(__uint_as_float(x[16 * kb + e]), __uint_as_float(x[16 * kb + e + 1])), cf2, add2));
+                                    float p0 = kd_exp2(y.x), p1 = kd_exp2(y.y);
+                                    sum2 = kp_add2(sum2, kp_two(p0, p1));
+                                    if (SPLIT) p0 *= fb[kb], p1 *= fb[kb];
+                                    const int at = k * 8 + (e >> 1);
+                                    hi[at] = kd_pack(p0, p1);
+                                    if (SPLIT) lo[at] = kd_pack_rest(p0, p1, hi[at]);
+                                }
+                                const float2 sum = kp_both(sum2);
+                                l += (sum.x + sum.y) * fl[kb];
+                            }
+                            KP_ST16(t_s + c + h * 32, hi);
+                            if (SPLIT) KP_ST16(t_s + c + h * 32 + 16, lo);
+                        }
                     }
                     kp_wait_st();
-                }
-                // factor of a block's scores; -infinity has to stay so in an edge tile: none of 0 or NaN there
-                auto factor = [&](int b) {
-                    float f = pr[b] * qs;
-                    if (edge) f = f < INFINITY ? fmaxf(f, 1e-30f) : 1e-30f;
-                    return f;
-                };
-                constexpr int CH = 32, NB = CH / 16;
-                float mt = -INFINITY, ut = -INFINITY;
-#pragma unroll 1
-                for (int c = 0; c < KT; c += CH) {
-                    uint32_t x[CH];
-#pragma unroll
-                    for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
-                    float f[NB];
-#pragma unroll
-                    for (int k = 0; k < NB; ++k) f[k] = factor(c / 16 + k);
-                    kp_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < NB; ++k) {
-                        float y = __uint_as_float(x[16 * k]);
-#pragma unroll
-                        for (int e = 1; e < 16; ++e) y = fmaxf(y, __uint_as_float(x[16 * k + e]));
-                        y *= f[k];
-                        mt = fmaxf(mt, y);
-                        ut = fmaxf(ut, y + pr[8 + c / 16 + k]);
+                    kp_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&p_full[s]);
+                        mbar_arrive(&prep_empty[slot]);
                     }
                 }
-                if (__any_sync(0xffffffffu, mt > m + KD_LAZY || ut > u + KD_LAZY)) {
-                    // each row by itself: what another row sees has no say
-                    const float mn = mt > m + KD_LAZY ? ceilf(mt) : m;
-                    const float un = fmaxf(ut > u + KD_LAZY ? ceilf(ut) : u, mn - KD_FLOOR);
-                    l *= mn == -INFINITY ? 1.f : kd_exp2(m - mn);
-                    const float al = un == -INFINITY ? 1.f : kd_exp2(u - un);
-                    m = mn, u = un;
-                    up = m == -INFINITY ? 0.f : KD_UP + m - u;
-                    down = kd_exp2(-up);
-                    if (have_o) {  // the products of the tiles before have ended: S came after them
-#pragma unroll 1
-                        for (int c = 0; c < HDO; c += 16) {
-                            uint32_t r[16];
-                            KP_LD16(r, t_o + c);
-                            kp_wait_ld();
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) r[e] = __float_as_uint(__uint_as_float(r[e]) * al);
-                            KP_ST16(t_o + c, r);
-                        }
-                    }
+                // ---- the end of the unit (or of this part), or of a turn
+                const bool end_of = j >= g.cnt;
+                if (end_of) {
+                    wait(o_full, n_o++);
+                } else {
+                    // the scores of this stream's next tile come after the products before them; without one the sums wait for the end
+                    const bool next = kp_active<SPLIT>(g, s, g.tile0 + j) || (SPLIT && j + 1 < g.cnt && kp_active<SPLIT>(g, s, g.tile0 + j + 1));
+                    if (!next || !have_o) continue;
+                    wait(&s_full[s], n_s);
                 }
-                have_o = true;
-                const float mm = m == -INFINITY ? 0.f : m;
-                // ---- weights, in place of the scores
-#pragma unroll 1
-                for (int c = 0; c < KT; c += CH) {
-                    uint32_t x[CH];
-#pragma unroll
-                    for (int k = 0; k < CH; k += 32) KP_LD32((x + k), t_s + c + k);
-                    float cf[NB], add[NB], fb[NB], fl[NB];
-#pragma unroll
-                    for (int k = 0; k < NB; ++k) {
-                        const int b = c / 16 + k;
-                        const float d = pr[8 + b] + up;
-                        const bool tiny = !(d >= -40.f);  // a page of zeros, or next to it for this row
-                        cf[k] = factor(b);
-                        add[k] = SPLIT ? -mm : (tiny ? -40.f : d) - mm;
-                        if ((bad >> b) & 1u) add[k] = __uint_as_float(0x7fffffffu);
-                        fb[k] = SPLIT ? (tiny ? 0.f : kd_exp2(fminf(d, 127.f))) : 0.f;
-                        fl[k] = SPLIT ? 1.f : tiny ? 1.0995116e12f : pr[16 + b] * down;
-                    }
-                    kp_wait_ld();
-#pragma unroll
-                    for (int h = 0; h < CH / 32; ++h) {
-                        uint32_t hi[16], lo[16];
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const int kb = 2 * h + k;
-                            const uint64_t cf2 = kp_two(cf[kb], cf[kb]), add2 = kp_two(add[kb], add[kb]);
-                            uint64_t sum2 = 0;
-#pragma unroll
-                            for (int e = 0; e < 16; e += 2) {
-                                const float2 y = kp_both(kp_fma2(
-                                    kp_two(__uint_as_float(x[16 * kb + e]), __uint_as_float(x[16 * kb + e + 1])), cf2, add2));
-                                float p0 = kd_exp2(y.x), p1 = kd_exp2(y.y);
-                                sum2 = kp_add2(sum2, kp_two(p0, p1));
-                                if (SPLIT) p0 *= fb[kb], p1 *= fb[kb];
-                                const int at = k * 8 + (e >> 1);
-                                hi[at] = kd_pack(p0, p1);
-                                if (SPLIT) lo[at] = kd_pack_rest(p0, p1, hi[at]);
-                            }
-                            const float2 sum = kp_both(sum2);
-                            l += (sum.x + sum.y) * fl[kb];
-                        }
-                        KP_ST16(t_s + c + h * 32, hi);
-                        if (SPLIT) KP_ST16(t_s + c + h * 32 + 16, lo);
-                    }
-                }
-                kp_wait_st();
-                kp_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&p_full[s]);
-                    mbar_arrive(&prep_empty[slot]);
-                }
-            }
-            // ---- the unit's (or this part's) end
-            wait(o_full, n_o++);
-            __syncwarp();
-            kp_fence_after();
-            const bool whole = g.cnt == g.tiles, direct = whole && !SPLIT;
-            const int c_first = (g.unit0 + KP_UNIT) / per, c_last = (g.unit0 + KP_UNIT + g.tiles - 1) / per;
-            if (SPLIT) {
-                drain();
-            } else {  // out, or to the record
-                const float mul = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+                kp_fence_after();
+                float mul = direct ? (l == 0.f ? 0.f : 1.f / l) : 1.f, f = 0.f;
+                float2* ml = reinterpret_cast<float2*>(record()) + row;
                 float4* rec = reinterpret_cast<float4*>(record() + 256) + row;
+                if (again) {
+                    const float2 v = __ldcg(ml);
+                    const float mn = fmaxf(m, v.x), mz = mn == -INFINITY ? 0.f : mn;
+                    mul = kd_exp2(m - mz), f = kd_exp2(v.x - mz);
+                    l = l * mul + v.y * f;
+                    m = mn;
+                }
 #pragma unroll 1
                 for (int c = 0; c < HDO; c += 16) {
                     uint32_t r[16];
@@ -948,15 +924,27 @@ __global__ void __launch_bounds__(KP_THREADS, 1)
                         }
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 16; e += 4)
-                            __stcg(rec + ((c + e) >> 2) * 128, make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                        for (int e = 0; e < 16; e += 4) {
+                            float4* at = rec + ((c + e) >> 2) * 128;
+                            if (again) {
+                                const float4 v = __ldcg(at);
+                                x[e] = fmaf(v.x, f, x[e]), x[e + 1] = fmaf(v.y, f, x[e + 1]);
+                                x[e + 2] = fmaf(v.z, f, x[e + 2]), x[e + 3] = fmaf(v.w, f, x[e + 3]);
+                            }
+                            __stcg(at, make_float4(x[e], x[e + 1], x[e + 2], x[e + 3]));
+                        }
                     }
                 }
+                if (!direct) __stcg(ml, make_float2(m, l));
+                if (end_of) break;
+                again = true, have_o = false;
+                m = u = -INFINITY, l = 0.f, up = 0.f, down = 1.f;
+                kp_fence_before();
             }
+            const int c_first = (g.unit0 + KP_UNIT) / per, c_last = (g.unit0 + KP_UNIT + g.tiles - 1) / per;
             if (direct) {
                 if (valid && a.lse && (!HALVES || s == 0)) a.lse[tok * a.n_q_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.693147180559945f;
             } else {
-                __stcg(reinterpret_cast<float2*>(record()) + row, make_float2(m, l));
                 __threadfence();
                 named_bar_sync(1, 256);
                 if (tid == 0) {

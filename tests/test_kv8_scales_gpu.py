@@ -142,3 +142,26 @@ def test_scales_at_the_ends_of_the_float_range(fb, T, ref, n, type):  # noqa: F8
         p = b.table[0][1]
         b.cache.v[p], b.cache.vs[p] = 0, 0
         check(b, ref)
+
+
+@pytest.mark.parametrize("type", [1, 2])
+@pytest.mark.parametrize("hq,hkv,hd", [(8, 1, 128), (4, 1, 64), (4, 1, 256)])
+def test_sums_over_very_many_keys_are_not_biased(fb, T, ref, type, hq, hkv, hd):  # noqa: F811
+    """131000 keys under many rows, so that a block of threads goes through all of them, positive values: the mean relative error,
+    in which roundings to nearest cancel, stays below half a step of the output type (2^-12 for fp16)."""
+    kv, n = 131000, 16384 if hd != 256 else 8192
+    b = Batch(fb, T, [(kv, n)], hq, hkv, hd, 64, 0, type, q_scale=0.5)
+    c = b.cache
+    c.v = c.v.view(T.int8).abs().view(T.uint8)
+    c.vs.fill_(2.0 ** -7)
+    out, _ = b.run()
+    ids = T.tensor(b.table[0][:-(-kv // 64)], device="cuda")
+    K = (ref.values(c.k[ids], 0) * c.ks[ids].double()[:, :, None, None])[:, 0].reshape(-1, hd)[:kv]
+    V = (ref.values(c.v[ids], 0) * 2.0 ** -7)[:, 0].reshape(-1, hd)[:kv]
+    off = []
+    for r0 in range(0, n, 2048):
+        rows = T.arange(r0, r0 + 32, device="cuda")
+        x = b.q.reshape(n, hq, hd)[rows, 3].double() @ K.T * b.scale
+        w = T.softmax(x.masked_fill(T.arange(kv, device="cuda") > (kv - n + rows)[:, None], -math.inf), 1) @ V
+        off.append((out.reshape(n, hq, hd)[rows, 3].double() - w) / w)
+    assert abs(T.cat(off).mean().item()) < 2.0 ** -12
