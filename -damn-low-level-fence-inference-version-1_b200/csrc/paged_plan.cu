@@ -88,6 +88,7 @@ __global__ void paged_plan_kernel(const PlanArgs p) {
         const int held = (int)(((long long)ctx + P - 1) >> sh);
         const int need = raw >= 0 && fits ? (int)((both + P - 1) >> sh) - held : 0;
         const int back = raw < 0 ? min(held, MP) : 0;
+        if (blockIdx.x == 0 && (b.ctx_len[r] < 0 || held > MP)) set_device_error(KV8_BAD);  // taken as 0; not placed
         s_ctx[r] = ctx;
         s_start[r] = nw;
         s_need[r] = need;

@@ -449,7 +449,7 @@ typedef struct fence_paged_batch { /* one step's batch; the plan's inputs and ou
     int n_pages;                   /* pages of the pool                                          */
     int n_touch;                   /* rows of touch: min(n_tokens, 2 n_req + n_tokens / page_tokens) */
     /* in */
-    const int* ctx_len;            /* [n_req] tokens each request has in the cache               */
+    const int* ctx_len;            /* [n_req] tokens each request has in the cache, at most max_pages * page_tokens */
     const int* new_len;            /* [n_req] tokens it brings now; negative: it has ended       */
     int* block_table;              /* [n_req][max_pages] page ids; the plan adds the new entries  */
     int* free_pages;               /* [n_pages] stack of free pages, entries 0 .. *n_free - 1    */
