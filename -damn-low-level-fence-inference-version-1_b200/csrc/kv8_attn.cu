@@ -70,7 +70,9 @@ static int kv8_launch_prefill(const KAttnArgs& p, cudaStream_t st) {
 constexpr size_t KV8_ARRIVED_BYTES = 4096;  // counters, at the workspace's start: 2048 for each kernel
 // The most query rows per KV head of a request that the decode kernel takes (16 in one pass over the keys, more in several).
 // Both kernels measured, heads 32/8 of 128, int8, bf16, us (decode / prefill kernel): 16 requests at 8000 keys 137 / 196 with
-// 32 rows, 257 / 197 with 64; at 30000 keys 449 / 587 and 881 / 585; one request at 1000 keys 19 / 37 and 20 / 38.
+// 32 rows, 257 / 197 with 64; at 30000 keys 449 / 587 and 881 / 585; one request at 1000 keys 19 / 37 and 20 / 38. The rule
+// goes by rows alone, so that the workspace and the launches follow from the shapes on the host: with few keys the prefill
+// kernel loses up to those 18 us. Heads of 64 and 256 and fp32 use the same border, unmeasured.
 constexpr int KV8_DECODE_ROWS = 48;
 
 // Whether the batch needs the prefill kernel.

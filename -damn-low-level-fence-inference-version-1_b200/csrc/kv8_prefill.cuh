@@ -5,15 +5,15 @@
 //
 // Bound: the matrix unit (4 head_dim operations per visible pair) and, as large here, the exponentials:
 // 128 x 128 of them per tile at 16 a clock take as long as the tile's products. 2048 rows of 32 heads of 128 at 30000
-// keys: 1.29 ms, 810 TFLOP/s (half of the measured matrix rate); what is left is the softmax's chain of latencies per tile.
+// keys: 1.29 ms, 804 TFLOP/s (half of the measured matrix rate); what is left is the softmax's chain of latencies per tile.
 //
-//  * Work is the list of 128-key tiles of every (request, KV head, group of query rows), cut into equal
-//    runs, one per CTA, as in the decode kernel: causal groups of any length fill all SMs alike. Units
+//  * Work is the list of 128-key tiles of every (request, KV head, group of query rows), cut into runs of
+//    equal cost, one per CTA, as in the decode kernel: causal groups of any length fill all SMs alike. Units
 //    that span CTAs are joined through the workspace in key order.
 //  * Rows of a group are (token, query head of the KV head): grouped heads share every K and V tile.
 //    Two streams of 128 rows per CTA take turns on the matrix unit: while one stream's softmax warps
 //    work, the other's products run. fp32 activations (SPLIT): one group of 128 rows, q and the weights as
-////    pairs of fp16, and the two streams take the even and the odd tiles. head_dim 256: both take every tile of
+//    pairs of fp16, and the two streams take the even and the odd tiles. head_dim 256: both take every tile of
 //    64 keys, and half the output channels (the scores are made twice: the sums of 256 channels fill two streams' space).
 //  * Codes become fp16 exactly, once per tile for both streams, by four converter warps, from stages that
 //    TMA fills a tile ahead, and stored as they lie, keys by channels, in 128-byte swizzled shared
@@ -22,7 +22,7 @@
 //    row are its own, as in the decode kernel.
 //  * S, then P in its place as fp16 (the weights are the A operand straight from tensor memory), and O
 //    stay in tensor memory: 2 x (128 + head_dim) of its 512 columns.
-//  * O is rescaled only when a row's maximum grows by more than 2^8 (fp16 weights have that room).
+//  * O is rescaled only when one of a row's references grows by more than 2^8 (fp16 weights have that room).
 #pragma once
 
 #include "kv8_decode.cuh"
