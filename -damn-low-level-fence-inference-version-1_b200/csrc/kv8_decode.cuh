@@ -61,7 +61,7 @@ constexpr int KD_MIN_TILES = 4;  // tiles per CTA below which more CTAs only add
 constexpr int KD_UNIT = 8;       // a unit's start and end cost about as much as eight tiles: counted so when the runs are cut
 constexpr float KD_LAZY = 8.f;   // the references may lag by 2^8
 constexpr float KD_UP = 6.f;     // weights enter fp16 times 2^6: below 2^(8 + 6 + 1), so small ones keep more of their bits
-constexpr float KD_FLOOR = 120.f;  // u >= m - 120, so that 2^(u - m) and its reciprocal are normal numbers: v_scale below that as if at it
+constexpr float KD_FLOOR = 120.f;  // u >= m - 120, so that 2^(u - m) and its reciprocal are normal numbers (for v_scale near 2^-126)
 
 template <int HD, bool SPLIT, int NT>
 struct KDShape {

@@ -165,3 +165,46 @@ def test_sums_over_very_many_keys_are_not_biased(fb, T, ref, type, hq, hkv, hd):
         w = T.softmax(x.masked_fill(T.arange(kv, device="cuda") > (kv - n + rows)[:, None], -math.inf), 1) @ V
         off.append((out.reshape(n, hq, hd)[rows, 3].double() - w) / w)
     assert abs(T.cat(off).mean().item()) < 2.0 ** -12
+
+
+def rows_of(b, ref, rows, heads):  # noqa: F811
+    """The definition for some rows of a request alone in its batch: (got - want, want, W) [rows][heads][head_dim or 1]."""
+    T, c, kv, n = b.T, b.cache, *b.lens[0]  # noqa: F811
+    ids = T.tensor(b.table[0][:-(-kv // c.page)], device="cuda")
+    G, at = b.hq // c.hkv, (kv - n + rows)[:, None]
+    key = T.arange(kv, device="cuda")
+    hide = (key > at) | (key <= at - b.window) if b.window > 0 else key > at
+    got, want, W = [], [], []
+    for h in heads:
+        K = (ref.values(c.k[ids, h // G], c.fmt) * c.ks[ids, h // G].double()[:, None, None]).reshape(-1, c.hd)[:kv]
+        V = (ref.values(c.v[ids, h // G], c.fmt) * c.vs[ids, h // G].double()[:, None, None]).reshape(-1, c.hd)[:kv]
+        x = b.q.reshape(n, b.hq, c.hd)[rows, h].double() @ K.T * b.scale
+        p = T.softmax(x.masked_fill(hide, -math.inf), 1)
+        want.append(p @ V)
+        W.append(p @ V.abs().amax(1, keepdim=True))
+        got.append(b.out.reshape(n, b.hq, c.hd)[rows, h].double())
+    return T.stack(got, 1) - T.stack(want, 1), T.stack(want, 1), T.stack(W, 1)
+
+
+@pytest.mark.parametrize("hd,hq,hkv,type", [(64, 32, 4, 1), (128, 64, 8, 2), (256, 16, 4, 1)])
+@pytest.mark.parametrize("window", [0, 33000])
+def test_parts_longer_than_the_sums_stay_in_one_place(fb, T, ref, hd, hq, hkv, type, window):  # noqa: F811
+    """Rows at positions around 32768 (with a window, from further on), where one half of a group of rows has a tile more than
+    the other: the sums leave tensor memory there."""
+    kv, n = (34816, 4096) if window == 0 else (70016, 4096)
+    b = Batch(fb, T, [(kv, n)], hq, hkv, hd, 128, 0, type, window=window, q_scale=2.0)
+    for j, p in enumerate(b.table[0][:kv // 128]):
+        b.cache.vs[p] *= 1 + j % 5
+    b.run()
+    rows = T.arange(2048 - 160, 2048 + 160, 3, device="cuda")
+    off, want, W = rows_of(b, ref, rows, (0, hq // 2 + 1, hq - 1))
+    tol = 2.0 ** -10 * W + (2.0 ** -10 if type == 1 else 2.0 ** -8) * want.abs()
+    assert bool((off.abs() <= tol).all()), (off.abs() / W).max().item()
+
+
+@pytest.mark.parametrize("window", [0, 900, 1100, 1500, 2600])
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64)])
+def test_fp32_rows_over_many_drains(fb, T, ref, hd, page, window):  # noqa: F811
+    """fp32 prompts and chunks of many tiles, with windows whose first and last tiles fall anywhere between two drains."""
+    lens = [(4000 + 128 * i + 37 * i, 60 + 11 * i) for i in range(8)]
+    check(Batch(fb, T, lens, 8, 2, hd, page, 0, 0, window=window, q_scale=2.0), ref)
